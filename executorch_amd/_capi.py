@@ -82,6 +82,26 @@ CHAIN_SIGNATURES = {
     "ets_logit_chain_last_error": (C.c_char_p, [C.c_void_p]),
 }
 
+
+class VerifyBatch(C.Structure):
+    """ets_verify_batch (include/et_speculative.h)."""
+
+    _fields_ = [("target_logits", C.c_void_p), ("draft_logits", C.c_void_p), ("dtype", C.c_int32), ("sequences", C.c_int32),
+                ("drafts", C.c_int32), ("temperature", C.c_float), ("target_sequence_stride", C.c_int64),
+                ("target_position_stride", C.c_int64), ("draft_sequence_stride", C.c_int64), ("draft_position_stride", C.c_int64),
+                ("draft_tokens", C.c_void_p), ("draft_tokens_stride", C.c_int64), ("draft_lengths", C.c_void_p),
+                ("temperatures", C.c_void_p), ("coins", C.c_void_p), ("coins_stride", C.c_int64), ("tokens", C.c_void_p),
+                ("tokens_stride", C.c_int64), ("accepted", C.c_void_p)]
+
+
+# every symbol declared in include/et_speculative.h
+SPECULATIVE_SIGNATURES = {
+    "ets_verifier_create": (C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_void_p)]),
+    "ets_verifier_destroy": (C.c_int32, [C.c_void_p]),
+    "ets_verifier_verify": (C.c_int32, [C.c_void_p, C.POINTER(VerifyBatch), C.c_void_p]),
+    "ets_verifier_last_error": (C.c_char_p, [C.c_void_p]),
+}
+
 # csrc/ets_test_hooks.h (libet_sampler_hooks.so)
 TEST_HOOKS = {
     "ets_test_signal_floor": (C.c_int32, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
@@ -118,7 +138,7 @@ def _load(path: str, tables) -> C.CDLL:
 def lib() -> C.CDLL:
     global _lib
     if _lib is None:
-        _lib = _load(LIB_PATH, (SIGNATURES, CHAIN_SIGNATURES))
+        _lib = _load(LIB_PATH, (SIGNATURES, CHAIN_SIGNATURES, SPECULATIVE_SIGNATURES))
     return _lib
 
 

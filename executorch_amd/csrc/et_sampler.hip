@@ -172,18 +172,6 @@ bool dtype_ok(int32_t dtype) {
 
 size_t dtype_size(int32_t dtype) { return dtype == ETS_DTYPE_FLOAT ? 4 : 2; }
 
-// Device guard: the handle's buffers live on the device that was current at creation.
-struct DeviceGuard {
-  int prev = -1;
-  bool switched = false;
-  explicit DeviceGuard(int dev) {
-    if (hipGetDevice(&prev) == hipSuccess && prev != dev) switched = (hipSetDevice(dev) == hipSuccess);
-  }
-  ~DeviceGuard() {
-    if (switched) (void)hipSetDevice(prev);
-  }
-};
-
 // ---- device timing ------------------------------------------------------------------------------
 ets_status harvest_timing_slot(ets_sampler* s, int slot) {
   if (!s->t_busy[slot]) return ETS_OK;

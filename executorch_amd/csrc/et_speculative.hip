@@ -1,0 +1,187 @@
+// Host side of include/et_speculative.h: the verification of drafted tokens.
+#include "../../include/et_speculative.h"
+
+#include <cmath>
+#include <cstdio>
+#include <new>
+
+#include "ets_host.h"
+#include "ets_verify.h"
+
+struct ets_verifier {
+  int32_t vocab = 0, max_sequences = 0, max_drafts = 0;
+  int device = 0;
+  ets::ChunkStat* d_stats = nullptr;  // [max_sequences, 2 max_drafts + 1, chunks of kSmallChunk]
+  double* d_rest = nullptr;           // [max_sequences, chunks of kSmallChunk]
+  double* d_exp2 = nullptr;           // 2^(j / kExp2Steps)
+  char last_error[256] = "";
+};
+
+namespace {
+
+thread_local char g_verifier_error[256] = "";
+
+ets_status verifier_fail(ets_verifier* v, ets_status code, const char* msg, const char* detail = nullptr) {
+  std::snprintf(v ? v->last_error : g_verifier_error, 256, "%s%s%s", msg, detail ? ": " : "", detail ? detail : "");
+  return code;
+}
+
+ets_status verifier_hip_fail(ets_verifier* v, hipError_t e, const char* what) {
+  return verifier_fail(v, e == hipErrorOutOfMemory ? ETS_MEMORY_ALLOCATION_FAILED : ETS_INTERNAL, what, hipGetErrorString(e));
+}
+
+int64_t chunks_of(int32_t vocab, int32_t chunk) { return (static_cast<int64_t>(vocab) + chunk - 1) / chunk; }
+
+bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+template <int DT, int CHUNK>
+hipError_t launch_verify(const ets::VerifyParams& p, hipStream_t stream) {
+  constexpr int U = CHUNK / (ets::kVerifyBlock * ets::VecElems<DT>::value);
+  const int64_t rows = static_cast<int64_t>(p.sequences) * p.rows_per_seq;
+  hipLaunchKernelGGL((ets::verify_stats_kernel<DT, U>), dim3(static_cast<uint32_t>(rows * p.chunks)), dim3(ets::kVerifyBlock), 0,
+                     stream, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if (p.draft) {
+    hipLaunchKernelGGL((ets::verify_rest_kernel<DT, U>), dim3(static_cast<uint32_t>(static_cast<int64_t>(p.sequences) * p.chunks)),
+                       dim3(ets::kVerifyBlock), 0, stream, p);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((ets::verify_finish_kernel<DT, CHUNK>), dim3(p.sequences), dim3(ets::kFinishBlock), 0, stream, p);
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_verify(ets::VerifyParams p, hipStream_t stream) {
+  // Large chunks when there are enough of them to fill the chip twice over, small ones otherwise.
+  const int64_t rows = static_cast<int64_t>(p.sequences) * p.rows_per_seq;
+  if (rows * chunks_of(p.vocab, ets::kLargeChunk) >= 512) {
+    p.chunks = static_cast<int32_t>(chunks_of(p.vocab, ets::kLargeChunk));
+    return launch_verify<DT, ets::kLargeChunk>(p, stream);
+  }
+  p.chunks = static_cast<int32_t>(chunks_of(p.vocab, ets::kSmallChunk));
+  return launch_verify<DT, ets::kSmallChunk>(p, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+ets_status ets_verifier_create(int32_t vocab_size, int32_t max_sequences, int32_t max_drafts, ets_verifier** out) {
+  if (!out) return verifier_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_verifier_create: out is null");
+  *out = nullptr;
+  if (vocab_size < 1) return verifier_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_verifier_create: vocab_size must be >= 1");
+  if (vocab_size >= (1 << 24)) return verifier_fail(nullptr, ETS_NOT_SUPPORTED, "ets_verifier_create: vocab_size must be below 16777216");
+  if (max_sequences < 1) return verifier_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_verifier_create: max_sequences must be >= 1");
+  if (max_drafts < 0) return verifier_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_verifier_create: max_drafts must be >= 0");
+  if (max_drafts > ets::kMaxDrafts) return verifier_fail(nullptr, ETS_NOT_SUPPORTED, "ets_verifier_create: max_drafts must be at most 64");
+  const int64_t chunks = chunks_of(vocab_size, ets::kSmallChunk);
+  if (max_sequences > 65535 || static_cast<int64_t>(max_sequences) * (2 * max_drafts + 1) * chunks > INT32_MAX)
+    return verifier_fail(nullptr, ETS_NOT_SUPPORTED, "ets_verifier_create: max_sequences x max_drafts x vocab_size is too large for one launch");
+  ets_verifier* v = new (std::nothrow) ets_verifier();
+  if (!v) return verifier_fail(nullptr, ETS_MEMORY_ALLOCATION_FAILED, "ets_verifier_create: out of host memory");
+  v->vocab = vocab_size;
+  v->max_sequences = max_sequences;
+  v->max_drafts = max_drafts;
+  auto bail = [&](hipError_t e, const char* what) {
+    const ets_status st = verifier_hip_fail(nullptr, e, what);
+    ets_verifier_destroy(v);
+    return st;
+  };
+  hipError_t e = hipGetDevice(&v->device);
+  if (e != hipSuccess) return bail(e, "ets_verifier_create: hipGetDevice");
+  const size_t rows = static_cast<size_t>(max_sequences) * (2 * max_drafts + 1);
+  e = hipMalloc(reinterpret_cast<void**>(&v->d_stats), rows * chunks * sizeof(ets::ChunkStat));
+  if (e != hipSuccess) return bail(e, "ets_verifier_create: hipMalloc(statistics)");
+  e = hipMalloc(reinterpret_cast<void**>(&v->d_rest), static_cast<size_t>(max_sequences) * chunks * sizeof(double));
+  if (e != hipSuccess) return bail(e, "ets_verifier_create: hipMalloc(residual masses)");
+  e = hipMalloc(reinterpret_cast<void**>(&v->d_exp2), ets::kExp2Steps * sizeof(double));
+  if (e != hipSuccess) return bail(e, "ets_verifier_create: hipMalloc(table)");
+  double table[ets::kExp2Steps];
+  for (int j = 0; j < ets::kExp2Steps; ++j) table[j] = std::exp2(static_cast<double>(j) / ets::kExp2Steps);
+  e = hipMemcpy(v->d_exp2, table, sizeof(table), hipMemcpyHostToDevice);
+  if (e != hipSuccess) return bail(e, "ets_verifier_create: hipMemcpy(table)");
+  *out = v;
+  return ETS_OK;
+}
+
+ets_status ets_verifier_destroy(ets_verifier* v) {
+  if (!v) return ETS_OK;
+  {
+    ets_host::DeviceGuard g(v->device);
+    (void)hipFree(v->d_stats);
+    (void)hipFree(v->d_rest);
+    (void)hipFree(v->d_exp2);
+  }
+  delete v;
+  return ETS_OK;
+}
+
+ets_status ets_verifier_verify(ets_verifier* v, const ets_verify_batch* a, void* hip_stream) {
+  if (!v) return verifier_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_verifier_verify: null handle");
+  v->last_error[0] = 0;
+  if (!a) return verifier_fail(v, ETS_INVALID_ARGUMENT, "ets_verifier_verify: null batch");
+  if (a->dtype != ETS_DTYPE_FLOAT && a->dtype != ETS_DTYPE_HALF && a->dtype != ETS_DTYPE_BFLOAT16)
+    return verifier_fail(v, ETS_INVALID_ARGUMENT, "ets_verifier_verify: element type must be Float, Half or BFloat16");
+  if (a->sequences < 0 || a->sequences > v->max_sequences)
+    return verifier_fail(v, ETS_INVALID_ARGUMENT, "ets_verifier_verify: sequences exceeds the handle's max_sequences");
+  if (a->drafts < 0 || a->drafts > v->max_drafts)
+    return verifier_fail(v, ETS_INVALID_ARGUMENT, "ets_verifier_verify: drafts exceeds the handle's max_drafts");
+  if (a->sequences == 0) return ETS_OK;
+  if (!a->target_logits || !a->coins || !a->tokens || !a->accepted || (a->drafts > 0 && !a->draft_tokens))
+    return verifier_fail(v, ETS_INVALID_ARGUMENT, "ets_verifier_verify: null pointer");
+  // rows may be apart by any distance that keeps them from overlapping; a dimension of extent 1 has no stride
+  const bool rows_apart = (a->drafts == 0 || a->target_position_stride >= v->vocab) &&
+                          (a->sequences == 1 || a->target_sequence_stride >= v->vocab);
+  if (!rows_apart) return verifier_fail(v, ETS_INVALID_ARGUMENT, "ets_verifier_verify: target strides smaller than vocab_size");
+  const bool with_draft = a->draft_logits && a->drafts > 0;
+  if (with_draft && !((a->drafts == 1 || a->draft_position_stride >= v->vocab) &&
+                      (a->sequences == 1 || a->draft_sequence_stride >= v->vocab)))
+    return verifier_fail(v, ETS_INVALID_ARGUMENT, "ets_verifier_verify: draft strides smaller than vocab_size");
+  if (a->sequences > 1 && (a->coins_stride < a->drafts + 1 || a->tokens_stride < a->drafts + 1 ||
+                           (a->drafts > 0 && a->draft_tokens_stride < a->drafts)))
+    return verifier_fail(v, ETS_INVALID_ARGUMENT, "ets_verifier_verify: row stride of tokens or coins too small");
+  const size_t elem = a->dtype == ETS_DTYPE_FLOAT ? 4 : 2;
+  if (!aligned_to(a->target_logits, elem) || (with_draft && !aligned_to(a->draft_logits, elem)) || !aligned_to(a->coins, 4) ||
+      !aligned_to(a->tokens, 4) || !aligned_to(a->accepted, 4) || !aligned_to(a->draft_tokens, 4) ||
+      !aligned_to(a->draft_lengths, 4) || !aligned_to(a->temperatures, 4))
+    return verifier_fail(v, ETS_INVALID_ARGUMENT, "ets_verifier_verify: pointer not aligned to its element type");
+  ets::VerifyParams p = {};
+  p.target = a->target_logits;
+  p.draft = with_draft ? a->draft_logits : nullptr;
+  p.target_seq = a->target_sequence_stride;
+  p.target_pos = a->target_position_stride;
+  p.draft_seq = a->draft_sequence_stride;
+  p.draft_pos = a->draft_position_stride;
+  p.draft_tokens = a->draft_tokens;
+  p.draft_tokens_stride = a->draft_tokens_stride;
+  p.lengths = a->draft_lengths;
+  p.temperatures = a->temperatures;
+  p.temperature = a->temperature;
+  p.coins = a->coins;
+  p.coins_stride = a->coins_stride;
+  p.tokens = a->tokens;
+  p.tokens_stride = a->tokens_stride;
+  p.accepted = a->accepted;
+  p.vocab = v->vocab;
+  p.drafts = a->drafts;
+  p.sequences = a->sequences;
+  p.rows_per_seq = p.draft ? 2 * a->drafts + 1 : a->drafts + 1;
+  p.stats = v->d_stats;
+  p.rest = v->d_rest;
+  p.exp2_table = v->d_exp2;
+  ets_host::DeviceGuard g(v->device);
+  hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+  hipError_t e = hipSuccess;
+  switch (a->dtype) {
+    case ETS_DTYPE_FLOAT: e = launch_verify<ets::kDtypeFloat>(p, stream); break;
+    case ETS_DTYPE_HALF: e = launch_verify<ets::kDtypeHalf>(p, stream); break;
+    default: e = launch_verify<ets::kDtypeBFloat16>(p, stream); break;
+  }
+  return e == hipSuccess ? ETS_OK : verifier_hip_fail(v, e, "ets_verifier_verify: launch");
+}
+
+const char* ets_verifier_last_error(const ets_verifier* v) { return v ? v->last_error : g_verifier_error; }
+
+}  // extern "C"

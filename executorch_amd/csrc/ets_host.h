@@ -106,6 +106,18 @@ constexpr int kMaxDevices = 64;
 // pass 2's LDS next to the expf table.
 constexpr int kPhistWordsHalf = 24576, kPhistWordsBFloat16 = 8192;
 
+// Device guard: the handle's buffers live on the device that was current at creation.
+struct DeviceGuard {
+  int prev = -1;
+  bool switched = false;
+  explicit DeviceGuard(int dev) {
+    if (hipGetDevice(&prev) == hipSuccess && prev != dev) switched = (hipSetDevice(dev) == hipSuccess);
+  }
+  ~DeviceGuard() {
+    if (switched) (void)hipSetDevice(prev);
+  }
+};
+
 // Records `msg` in the handle (or, without one, for the calling thread) and returns `code`.
 ets_status fail(ets_sampler* s, ets_status code, const std::string& msg);
 ets_status hip_fail(ets_sampler* s, hipError_t e, const char* what);

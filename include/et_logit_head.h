@@ -1,0 +1,64 @@
+/*
+ * et_logit_head.h -- C ABI of the logits head with 4-bit weights (MI355X, gfx950).
+ *
+ * The last layer in front of the sampler: hidden states [rows, hidden] times a [vocab, hidden] matrix of
+ * 4-bit weights with a scale (and, where given, a zero) per group of columns:
+ *
+ *   logits[m, v] = sum_k x[m, k] * w[v, k]
+ *   w[v, k] = (n[v, k] - 8) * scale[v, k / group] + zero[v, k / group],   n[v, k] in 0 .. 15
+ *
+ * Two weights share a byte: column 2j is the low nibble of byte j of its row, column 2j + 1 the high one.
+ * The products are exact (n - 8 is a small integer) and summed in fp32, scales and zeros are applied in
+ * fp32 per group, and the logits are rounded once, to the type asked for.  A row of x that holds an
+ * infinity or a NaN gives no finite logits.
+ *
+ * Nothing in the reference's sampler corresponds to this: there the logits come out of the exported
+ * program.  Status codes and dtype codes are those of et_sampler.h.
+ */
+#ifndef ET_LOGIT_HEAD_H_
+#define ET_LOGIT_HEAD_H_
+
+#include "et_sampler.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+typedef struct ets_logit_head ets_logit_head;
+
+/* Lays the weights out for the kernels in memory of its own on the current HIP device (as large as the
+ * packed weights, rounded up to 16 rows x 128 columns, plus the scales) and waits for `hip_stream`, so
+ * the caller may free its own copy when the call returns.  All pointers are DEVICE pointers:
+ *   d_packed  uint8 [vocab, (hidden + 1) / 2], rows `packed_stride` bytes apart
+ *   d_scales  [vocab, ceil(hidden / group)] of `scale_dtype` (Float, Half or BFloat16), contiguous
+ *   d_zeros   the same shape and type, or NULL for symmetric weights
+ * group_size: 32, 64 or a multiple of 128 (the last group of a row may be cut short by `hidden`; a group
+ * at least as long as the row is one scale per row). */
+ETS_API ets_status ets_logit_head_create(int32_t vocab_size, int32_t hidden_size, int32_t group_size, const void* d_packed,
+                                         int64_t packed_stride, const void* d_scales, const void* d_zeros,
+                                         int32_t scale_dtype, void* hip_stream, ets_logit_head** out);
+ETS_API ets_status ets_logit_head_destroy(ets_logit_head* h);
+
+/* Logits of `rows` hidden states, asynchronously on `hip_stream`; allocates nothing, may be captured.
+ * d_hidden: [rows, hidden] of `dtype`, d_logits: [rows, vocab] of `logits_dtype` (each Float, Half or
+ * BFloat16), rows the given numbers of elements apart (innermost stride 1).  Calls on one handle only
+ * read it, so they may overlap on several streams. */
+ETS_API ets_status ets_logit_head_logits(ets_logit_head* h, const void* d_hidden, int32_t dtype, int32_t rows,
+                                         int64_t hidden_stride, void* d_logits, int32_t logits_dtype, int64_t logits_stride,
+                                         void* hip_stream);
+
+/* Hidden states to tokens: ets_logit_head_logits() into the caller's `d_logits`, then
+ * ets_sampler_sample_batch() on them, on one stream.  The head's vocabulary must be the sampler's, and
+ * both must live on one device.  Errors are reported on the sampler's handle. */
+ETS_API ets_status ets_sampler_sample_hidden(ets_sampler* s, ets_logit_head* h, const void* d_hidden, int32_t dtype,
+                                             int32_t rows, int64_t hidden_stride, void* d_logits, int32_t logits_dtype,
+                                             int64_t logits_stride, int32_t* d_tokens, void* hip_stream);
+
+/* Text of the last error on this handle (NULL: of the calling thread's last failed create). */
+ETS_API const char* ets_logit_head_last_error(const ets_logit_head* h);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* ET_LOGIT_HEAD_H_ */

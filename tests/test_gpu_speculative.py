@@ -1,0 +1,332 @@
+"""DraftVerifier through the C ABI against the float64 restatement: tokens and counts must be equal.
+(The kernels hold weights and sums to about 1e-13 in 64 bits, so a coin would have to fall within about
+1e-11 of a border for the two to differ: for the draws here a chance below 1e-6 in all.)"""
+import numpy as np
+import pytest
+import torch
+
+import executorch_amd as ea
+from executorch_amd import _capi
+from oracle import verify_oracle as VO
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def problem(seed, S, K, V, dtype, dev, draft=True, ragged=False, pad=0, temps=(0.0, 0.3, 0.7, 1.0, 1.7), sharp=6.0):
+    """Inputs on the device: rows `pad` entries longer than the vocabulary, drafts drawn from the draft rows."""
+    g = np.random.default_rng(seed)
+    t = g.standard_normal((S, K + 1, V + pad)).astype(np.float32)
+    for b in range(S):
+        for i in range(K + 1):
+            t[b, i, g.integers(0, V, size=min(V, 12))] += sharp
+    d = (t[:, :K] + 0.6 * g.standard_normal((S, K, V + pad))).astype(np.float32)
+    temperature = np.asarray(temps, np.float32)[g.integers(0, len(temps), size=S)]
+    heat = np.where(temperature > 0, temperature, 1.0)[:, None, None]
+    tokens = (d[:, :, :V] + heat * g.gumbel(size=(S, K, V))).argmax(2) if K else np.zeros((S, 0))
+    if K and S > 1:  # greedy sequences see the arg-max now and then
+        rows = g.random((S, K)) < 0.5
+        tokens = np.where(rows & (temperature == 0)[:, None], t[:, :K, :V].argmax(2), tokens)
+    out = {"target": torch.from_numpy(t).to(dev).to(DT[dtype])[:, :, :V],
+           "draft": torch.from_numpy(d).to(dev).to(DT[dtype])[:, :, :V] if draft else None,
+           "tokens": torch.from_numpy(tokens.astype(np.int32)).to(dev),
+           "coins": torch.from_numpy(g.random((S, K + 1), dtype=np.float32)).to(dev),
+           "lengths": torch.from_numpy(g.integers(0, K + 1, size=S).astype(np.int32)).to(dev) if ragged else None,
+           "temperature": torch.from_numpy(temperature).to(dev)}
+    return out
+
+
+def want(x):
+    host = lambda t: None if t is None else t.float().cpu().numpy()  # noqa: E731
+    return VO.verify(host(x["target"]), host(x["draft"]), x["tokens"].cpu().numpy(), None if x["lengths"] is None else x["lengths"].cpu().numpy(),
+                     x["temperature"].cpu().numpy(), x["coins"].cpu().numpy())
+
+
+def call(v, x, **more):
+    return v.verify(x["target"], x["tokens"], x["coins"], draft_logits=x["draft"], draft_lengths=x["lengths"],
+                    temperature=x["temperature"], **more)
+
+
+def check(v, x, label):
+    tokens, accepted = call(v, x)
+    t, a = want(x)
+    assert np.array_equal(accepted.cpu().numpy(), a), (label, accepted.cpu().numpy(), a)
+    assert np.array_equal(tokens.cpu().numpy(), t), (label, tokens.cpu().numpy(), t)
+    return a
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 8, 9, 63, 255, 2047, 2048, 2049, 5000, 8191, 8193, 32000])
+def test_small_and_odd_vocabularies(dev, dtype, draft, vocab):
+    for K, S, pad in ((1, 1, 0), (3, 5, 3), (0, 2, 1)):
+        v = ea.DraftVerifier(vocab, S, K)
+        check(v, problem(vocab * 7 + K, S, K, vocab, dtype, dev, draft=draft, pad=pad), (dtype, draft, vocab, K))
+
+
+@pytest.mark.parametrize("dtype,S,K,V,draft,ragged,pad", [
+    ("bf16", 16, 4, 128256, True, False, 0), ("bf16", 24, 4, 128256, True, True, 5), ("f16", 7, 7, 151936, True, True, 1),
+    ("f32", 3, 5, 50257, True, False, 0), ("bf16", 5, 8, 262144, False, False, 0), ("f32", 2, 64, 4001, True, True, 0),
+    ("f16", 1, 64, 2500, False, False, 0), ("bf16", 64, 2, 32000, False, True, 8)])
+def test_serving_sizes(dev, dtype, S, K, V, draft, ragged, pad):
+    v = ea.DraftVerifier(V, S, K)
+    kept = [check(v, problem(100 + r, S, K, V, dtype, dev, draft=draft, ragged=ragged, pad=pad), (dtype, S, K, V, r)) for r in range(2)]
+    assert S == 1 or 0 < np.concatenate(kept).sum()  # the case is not vacuous (one sequence alone may keep none)
+
+
+def test_smaller_calls_of_a_larger_handle(dev):
+    v = ea.DraftVerifier(32000, 40, 8)
+    for S, K in ((40, 8), (1, 1), (3, 0), (40, 2), (7, 8)):
+        check(v, problem(S * 9 + K, S, K, 32000, "bf16", dev, ragged=K > 2), (S, K))
+    x = problem(1, 4, 2, 32000, "bf16", dev)
+    empty = {k: (None if t is None else t[:0]) for k, t in x.items()}
+    tokens, accepted = call(v, empty)
+    assert tokens.shape == (0, 3) and accepted.shape == (0,)
+
+
+@pytest.mark.parametrize("V", [2048, 8192, 65536])
+def test_borders_are_exact(dev, V):
+    """Equal logits: every weight is exactly 1, p exactly 1/V, so the comparisons are those of the formulas."""
+    S = 64
+    g = np.random.default_rng(V)
+    v = ea.DraftVerifier(V, S, 1)
+    target = torch.full((S, 2, V), 0.25, dtype=torch.bfloat16, device=dev)
+    drafted = g.integers(0, V, size=(S, 1)).astype(np.int32)
+    cell = g.integers(0, V, size=S)
+    cell[:4] = (0, V - 1, V // 2, 1)
+    coins = np.zeros((S, 2), np.float32)
+    coins[0::2, 0] = 1.0 / V  # coin * 1 < 1 / V fails by nothing
+    coins[1::2, 0] = np.nextafter(np.float32(1.0 / V), np.float32(0))
+    coins[:, 1] = cell / V
+    tokens, accepted = v.verify(target, torch.from_numpy(drafted).to(dev), torch.from_numpy(coins).to(dev), temperature=0.5)
+    assert accepted.cpu().tolist() == [0, 1] * (S // 2)
+    tokens = tokens.cpu().numpy()
+    assert np.array_equal(tokens[1::2, 1], cell[1::2])  # (v + 1) / V > cell / V first at v = cell
+    # without the drafted token V - 1 entries are left: entry v of them is drawn for floor(coin (V - 1)) == v
+    rank = np.floor(coins[0::2, 1].astype(np.float64) * (V - 1)).astype(np.int64)
+    assert np.array_equal(tokens[0::2, 0], rank + (rank >= drafted[0::2, 0]))
+    # two equal models: accepted whenever the coin is below 1, and nothing is left of p - q (drawn from p)
+    same = v.verify(target, torch.full((S, 1), V, dtype=torch.int32, device=dev), torch.from_numpy(coins).to(dev),
+                    draft_logits=target[:, :1], temperature=0.5)
+    assert same[1].sum().item() == 0 and np.array_equal(same[0].cpu().numpy()[:, 0], cell)
+    same = v.verify(target, torch.from_numpy(drafted).to(dev), torch.full((S, 2), 1 - 2.0 ** -24, device=dev),
+                    draft_logits=target[:, :1], temperature=0.5)
+    assert same[1].sum().item() == S
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("draft", [True, False])
+def test_masked_rows_and_rows_without_a_distribution(dev, dtype, draft):
+    S, K, V = 12, 2, 9000
+    x = problem(3, S, K, V, dtype, dev, draft=draft, temps=(0.8,))
+    lowest = torch.finfo(DT[dtype]).min
+    x["target"][0, :, 1:] = -float("inf")           # one token is left: nothing else can come out
+    x["target"][1, :, : V // 2] = -float("inf")     # half of the rows masked, chunks without an entry among them
+    x["target"][2, 0, :] = -float("inf")            # no token at all
+    x["target"][3, 0, V - 1] = float("nan")
+    x["target"][4, 0, 8500] = float("inf")
+    x["target"][5, :, 100:] = lowest                # masked by the type's lowest value
+    x["target"][6, :] = lowest                      # every entry the lowest value: an even distribution
+    x["temperature"][7] = float("nan")
+    if draft:
+        x["draft"][8, 0, :] = -float("inf")
+        x["draft"][9, 0, 5] = float("nan")
+        x["draft"][10, :, 100:] = -float("inf")
+    x["tokens"][11, 0] = -3                         # no token
+    x["tokens"][11, 1] = V
+    check(ea.DraftVerifier(V, S, K), x, (dtype, draft))
+    tokens, accepted = call(ea.DraftVerifier(V, S, K), x)
+    assert tokens[2, 0].item() == -1 and tokens[3, 0].item() == -1 and tokens[4, 0].item() == -1 and tokens[7, 0].item() == -1
+    # the same rows read greedily: +inf is the arg-max, NaN never
+    x["temperature"][:] = 0.0
+    check(ea.DraftVerifier(V, S, K), x, (dtype, draft, "greedy"))
+
+
+def test_odd_coins_and_temperatures(dev):
+    S, K, V = 10, 3, 5003
+    x = problem(17, S, K, V, "f32", dev)
+    x["coins"][0, :] = 0.0
+    x["coins"][1, :] = 1.0
+    x["coins"][2, :] = float("nan")
+    x["coins"][3, :] = -1.0
+    x["coins"][4, :] = 2.0
+    x["temperature"][:] = torch.tensor([0.7, 0.7, 0.7, 0.7, 0.7, 1e-30, 1e30, float("inf"), -2.0, 1e-45], device=dev)
+    t, a = VO.verify(x["target"].cpu().numpy(), x["draft"].cpu().numpy(), x["tokens"].cpu().numpy(), None,
+                     x["temperature"].cpu().numpy(), x["coins"].cpu().numpy())
+    got = call(ea.DraftVerifier(V, S, K), x)
+    assert np.array_equal(got[1].cpu().numpy(), a) and np.array_equal(got[0].cpu().numpy(), t)
+
+
+def test_what_lies_behind_a_length_is_not_read_and_outputs_beside_are_kept(dev):
+    S, K, V = 6, 4, 10001
+    x = problem(23, S, K, V, "bf16", dev, temps=(0.9,))
+    lengths = np.array([0, 1, 2, 3, 4, 9], np.int32)  # (9: clamped to K)
+    x["lengths"] = torch.from_numpy(lengths).to(dev)
+    for b in range(S):
+        x["target"][b, min(lengths[b], K) + 1:] = float("nan")
+        x["draft"][b, lengths[b]:] = float("nan")
+        x["tokens"][b, lengths[b]:] = 1 << 30
+        x["coins"][b, lengths[b]:K] = float("nan")
+    v = ea.DraftVerifier(V, S + 3, K)
+    wide = torch.full((S + 3, K + 4), 77, dtype=torch.int32, device=dev)
+    count = torch.full((S + 3,), 77, dtype=torch.int32, device=dev)
+    call(v, x, tokens_out=wide[:S, 1:K + 2], accepted_out=count[:S])
+    t, a = want(x)
+    assert np.array_equal(wide[:S, 1:K + 2].cpu().numpy(), t) and np.array_equal(count[:S].cpu().numpy(), a)
+    assert (wide[S:] == 77).all() and (wide[:, 0] == 77).all() and (wide[:, K + 2:] == 77).all() and (count[S:] == 77).all()
+    # a negative length is none
+    x["lengths"][:] = -5
+    x["target"] = x["target"][:, :1].expand(S, K + 1, V).contiguous()
+    check(v, x, "negative")
+
+
+def test_rows_apart_and_misaligned(dev):
+    """Strides of every kind: position-major rows, rows that start at odd elements, one row for all."""
+    S, K, V = 4, 3, 4099
+    for dtype in ("f16", "f32"):
+        x = problem(31, S, K, V, dtype, dev, temps=(0.7,))
+        v = ea.DraftVerifier(V, S, K)
+        t, a = want(x)
+        flat = torch.zeros((K + 1) * S * (V + 6) + 3, dtype=DT[dtype], device=dev)
+        view = flat[3:].view(K + 1, S, V + 6)[:, :, 2:2 + V].transpose(0, 1)
+        view.copy_(x["target"])
+        got = call(v, {**x, "target": view})
+        assert np.array_equal(got[0].cpu().numpy(), t) and np.array_equal(got[1].cpu().numpy(), a)
+        drafts = torch.zeros((S, K + 2), dtype=torch.int32, device=dev)
+        drafts[:, 1:K + 1] = x["tokens"]
+        coins = torch.zeros((S, K + 9), device=dev)
+        coins[:, 3:K + 4] = x["coins"]
+        got = call(v, {**x, "tokens": drafts[:, 1:K + 1], "coins": coins[:, 3:K + 4]})
+        assert np.array_equal(got[0].cpu().numpy(), t)
+        # the drafts' own memory may take the answer
+        tokens = torch.zeros((S, K + 1), dtype=torch.int32, device=dev)
+        tokens[:, :K] = x["tokens"]
+        got = call(v, {**x, "tokens": tokens[:, :K]}, tokens_out=tokens)
+        assert np.array_equal(tokens.cpu().numpy(), t)
+
+
+def test_rows_further_than_31_bits_apart(dev):
+    S, K, V = 2, 1, 70000
+    far = (1 << 31) // 2 + 12345  # elements of 2 bytes between positions: more than 2^31 bytes, sequences 2^32 apart
+    flat = torch.zeros(3 * far + V, dtype=torch.float16, device=dev)
+    x = problem(41, S, K, V, "f16", dev, temps=(0.8,))
+    view = flat.as_strided((S, K + 1, V), (2 * far, far, 1))
+    view.copy_(x["target"])
+    got = call(ea.DraftVerifier(V, S, K), {**x, "target": view})
+    t, a = want(x)
+    assert np.array_equal(got[0].cpu().numpy(), t) and np.array_equal(got[1].cpu().numpy(), a)
+
+
+def test_greedy_gives_the_samplers_arg_max(dev):
+    S, K, V = 9, 4, 32000
+    x = problem(51, S, K, V, "bf16", dev, draft=False, temps=(0.0,))
+    x["target"][:, :, 777] = x["target"].amax(2)  # ties
+    best = ea.Sampler(V, 0.0, 0.9, 1, max_batch=S * (K + 1)).sample_batch(x["target"].reshape(-1, V)).view(S, K + 1)
+    x["tokens"] = best[:, :K].clone().contiguous()
+    tokens, accepted = call(ea.DraftVerifier(V, S, K), x)
+    assert torch.equal(tokens, best) and (accepted == K).all()
+    x["tokens"][:, 2] += 1
+    tokens, accepted = call(ea.DraftVerifier(V, S, K), x)
+    assert (accepted == 2).all() and torch.equal(tokens[:, :3], best[:, :3]) and (tokens[:, 3:] == -1).all()
+
+
+def test_drafts_of_the_sampler_verified_have_the_targets_distribution(dev):
+    """The loop as it is used: draft tokens from Sampler (multinomial), verified; the first token of the
+    answers is distributed as the target's probabilities."""
+    V, S = 5, 4000
+    p_logits, q_logits = torch.tensor([1.0, 0.2, -0.5, 0.9, -2.0]), torch.tensor([0.0, 1.0, 0.3, -1.0, 0.5])
+    target = p_logits.to(dev).expand(S, 2, V).contiguous()
+    draft = q_logits.to(dev).expand(S, 1, V).contiguous()
+    smp = ea.Sampler(V, 1.0, 1.0, 99, max_batch=S)
+    v = ea.DraftVerifier(V, S, 1)
+    g = torch.Generator(device=dev)
+    g.manual_seed(7)
+    counts, N = np.zeros(V), 0
+    for _ in range(10):
+        x = smp.sample_batch(draft[:, 0]).view(S, 1)
+        tokens, _ = v.verify(target, x, torch.rand((S, 2), generator=g, device=dev), draft_logits=draft)
+        counts += np.bincount(tokens[:, 0].cpu().numpy(), minlength=V)
+        N += S
+    p = VO.probabilities(p_logits.numpy(), 1.0)
+    assert (np.abs(counts - N * p) < 5 * np.sqrt(N * p * (1 - p))).all(), (counts / N, p)
+
+
+def test_another_stream_and_two_handles_at_once(dev):
+    x, y = problem(61, 8, 4, 128256, "bf16", dev), problem(62, 5, 3, 50001, "f32", dev)
+    vx, vy = ea.DraftVerifier(128256, 8, 4), ea.DraftVerifier(50001, 5, 3)
+    wx, wy = want(x), want(y)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(a):
+            got.append((call(vx, x), wx))
+        with torch.cuda.stream(b):
+            got.append((call(vy, y), wy))
+    torch.cuda.synchronize()
+    for (tokens, accepted), (t, n) in got:
+        assert np.array_equal(tokens.cpu().numpy(), t) and np.array_equal(accepted.cpu().numpy(), n)
+
+
+def test_captured_and_replayed(dev):
+    S, K, V = 6, 4, 32000
+    v = ea.DraftVerifier(V, S, K)
+    x = problem(71, S, K, V, "bf16", dev, ragged=True)
+    tokens = torch.empty((S, K + 1), dtype=torch.int32, device=dev)
+    accepted = torch.empty(S, dtype=torch.int32, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(v, x, tokens_out=tokens, accepted_out=accepted)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(v, x, tokens_out=tokens, accepted_out=accepted)
+    for r in range(4):
+        fresh = problem(80 + r, S, K, V, "bf16", dev, ragged=True)
+        for name, t in x.items():
+            t.copy_(fresh[name])
+        tokens.fill_(-9)
+        graph.replay()
+        torch.cuda.synchronize()
+        t, a = want(fresh)
+        assert np.array_equal(tokens.cpu().numpy(), t) and np.array_equal(accepted.cpu().numpy(), a), r
+        check(v, fresh, ("eager between replays", r))
+
+
+def test_the_same_call_gives_the_same_answer(dev):
+    x = problem(91, 32, 4, 128256, "bf16", dev)
+    v = ea.DraftVerifier(128256, 32, 4)
+    first = call(v, x)
+    for _ in range(5):
+        again = call(v, x)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def test_refusals(dev):
+    S, K, V = 3, 2, 100
+    v = ea.DraftVerifier(V, S, K)
+    x = problem(5, S, K, V, "f32", dev)
+    bad = {
+        "type": {"target": x["target"].double()}, "draft type": {"draft": x["draft"].half()}, "vocab": {"target": x["target"][:, :, :-1]},
+        "positions": {"target": x["target"][:, :2]}, "draft shape": {"draft": x["draft"][:, :1]}, "tokens type": {"tokens": x["tokens"].long()},
+        "coins type": {"coins": x["coins"].double()}, "coins shape": {"coins": x["coins"][:, :2]}, "host": {"coins": x["coins"].cpu()},
+        "inner stride": {"target": torch.zeros((S, K + 1, 2 * V), device=dev)[:, :, ::2]}, "lengths": {"lengths": x["tokens"][0, :1]},
+        "lengths type": {"lengths": torch.zeros(S, device=dev)}, "temperature": {"temperature": torch.ones(S + 1, device=dev)},
+        "temperature type": {"temperature": torch.ones(S, device=dev).double()}, "overlap": {"target": torch.zeros((1, 1, V), device=dev).expand(S, K + 1, V)},
+        "rank": {"tokens": x["tokens"][0]}, "uint16": {"target": x["target"].to(torch.int16).view(torch.uint16), "draft": None},
+    }
+    for name, change in bad.items():
+        with pytest.raises(ea.SamplerError) as e:
+            call(v, {**x, **change})
+        assert e.value.code == _capi.INVALID_ARGUMENT, name
+    too_many = problem(6, S + 1, K, V, "f32", dev)
+    with pytest.raises(ea.SamplerError, match="max_sequences"):
+        call(v, too_many)
+    with pytest.raises(ea.SamplerError, match="max_drafts"):
+        call(v, problem(6, S, K + 1, V, "f32", dev))
+    for out in ({"tokens_out": torch.zeros((S, K), dtype=torch.int32, device=dev)}, {"accepted_out": torch.zeros(S, device=dev)}):
+        with pytest.raises(ea.SamplerError):
+            call(v, x, **out)
+    check(v, x, "the handle still works")
