@@ -102,6 +102,18 @@ SPECULATIVE_SIGNATURES = {
     "ets_verifier_last_error": (C.c_char_p, [C.c_void_p]),
 }
 
+# every symbol declared in include/et_logit_head.h
+HEAD_SIGNATURES = {
+    "ets_logit_head_create": (C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32,
+                              C.c_void_p, C.POINTER(C.c_void_p)]),
+    "ets_logit_head_destroy": (C.c_int32, [C.c_void_p]),
+    "ets_logit_head_logits": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_void_p, C.c_int32, C.c_int64,
+                              C.c_void_p]),
+    "ets_sampler_sample_hidden": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_void_p, C.c_int32,
+                                  C.c_int64, C.c_void_p, C.c_void_p]),
+    "ets_logit_head_last_error": (C.c_char_p, [C.c_void_p]),
+}
+
 # csrc/ets_test_hooks.h (libet_sampler_hooks.so)
 TEST_HOOKS = {
     "ets_test_signal_floor": (C.c_int32, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
@@ -138,7 +150,7 @@ def _load(path: str, tables) -> C.CDLL:
 def lib() -> C.CDLL:
     global _lib
     if _lib is None:
-        _lib = _load(LIB_PATH, (SIGNATURES, CHAIN_SIGNATURES, SPECULATIVE_SIGNATURES))
+        _lib = _load(LIB_PATH, (SIGNATURES, CHAIN_SIGNATURES, SPECULATIVE_SIGNATURES, HEAD_SIGNATURES))
     return _lib
 
 

@@ -55,6 +55,7 @@ LIB_UNITS = [
     "ets_split_f32.hip", "ets_split_f16.hip", "ets_split_bf16.hip",
     "ets_split_topk_f32.hip", "ets_split_topk_f16.hip", "ets_split_topk_bf16.hip",
     "et_speculative.hip",
+    "et_logit_head.hip", "ets_head_f32.hip", "ets_head_f16.hip", "ets_head_bf16.hip",
 ]
 # Test and measurement hooks (csrc/ets_test_hooks.h): a library of their own.
 HOOKS_LIB = os.path.join(HERE, "libet_sampler_hooks.so")

@@ -1,0 +1,242 @@
+// Host side of include/et_logit_head.h: the logits head with 4-bit weights.
+#include "../../include/et_logit_head.h"
+
+#include <algorithm>
+#include <cstdio>
+#include <new>
+
+#include "ets_head_launch.h"
+#include "ets_host.h"
+
+namespace ets {
+
+// ---- layout -------------------------------------------------------------------------------------
+// One lane per dword of the blocks.  Columns and rows that do not exist hold n = 8, the weight 0.
+__global__ void __launch_bounds__(kHeadBlock)
+head_layout_kernel(const uint8_t* packed, int64_t stride, int32_t vocab, int32_t hidden, int32_t chunks, int64_t dwords,
+                   uint32_t* blocks) {
+  for (int64_t d = static_cast<int64_t>(blockIdx.x) * kHeadBlock + threadIdx.x; d < dwords;
+       d += static_cast<int64_t>(gridDim.x) * kHeadBlock) {
+    const int t = static_cast<int>(d & 3), lane = static_cast<int>((d >> 2) & 63);
+    const int64_t block = d >> 8, tile = block / chunks;
+    const int chunk = static_cast<int>(block - tile * chunks);
+    const int64_t v = tile * kTileRows + (lane & 15);
+    const int k = chunk * kChunkCols + 32 * t + 8 * (lane >> 4);
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t nibble = 8;
+      if (v < vocab && k + j < hidden) nibble = (packed[v * stride + ((k + j) >> 1)] >> (4 * (j & 1))) & 15u;
+      w |= nibble << (16 * (j & 1) + 4 * (j >> 1));
+    }
+    blocks[d] = w;
+  }
+}
+
+// One lane per scale (or zero) of the layout; groups and rows that do not exist hold 0.
+template <typename T>
+__global__ void __launch_bounds__(kHeadBlock)
+head_scales_kernel(const T* scales, int32_t vocab, int32_t groups, int32_t per_chunk, int64_t per_tile, int64_t count, T* out) {
+  for (int64_t d = static_cast<int64_t>(blockIdx.x) * kHeadBlock + threadIdx.x; d < count;
+       d += static_cast<int64_t>(gridDim.x) * kHeadBlock) {
+    const int64_t tile = d / per_tile;
+    const int64_t in_tile = d - tile * per_tile;
+    const int64_t of = in_tile / (kTileRows * per_chunk);  // chunk, or group of 128 columns and more
+    const int rest = static_cast<int>(in_tile - of * (kTileRows * per_chunk));
+    const int64_t v = tile * kTileRows + rest / per_chunk, group = of * per_chunk + rest % per_chunk;
+    out[d] = (v < vocab && group < groups) ? scales[v * groups + group] : static_cast<T>(0);
+  }
+}
+
+}  // namespace ets
+
+struct ets_logit_head {
+  int32_t vocab = 0, hidden = 0;
+  int device = 0;
+  int32_t tiles = 0, chunks = 0, chunks_per_group = 1, groups = 0;
+  ets_host::HeadForm form = {};
+  bool scale_is_bf16 = false;
+  void* d_blocks = nullptr;
+  void* d_scales = nullptr;
+  void* d_zeros = nullptr;
+  char last_error[256] = "";
+};
+
+namespace {
+
+thread_local char g_head_error[256] = "";
+
+ets_status head_fail(ets_logit_head* h, ets_status code, const char* msg, const char* detail = nullptr) {
+  std::snprintf(h ? h->last_error : g_head_error, 256, "%s%s%s", msg, detail ? ": " : "", detail ? detail : "");
+  return code;
+}
+
+ets_status head_hip_fail(ets_logit_head* h, hipError_t e, const char* what) {
+  return head_fail(h, e == hipErrorOutOfMemory ? ETS_MEMORY_ALLOCATION_FAILED : ETS_INTERNAL, what, hipGetErrorString(e));
+}
+
+bool head_dtype(int32_t dtype) {
+  return dtype == ETS_DTYPE_FLOAT || dtype == ETS_DTYPE_HALF || dtype == ETS_DTYPE_BFLOAT16;
+}
+size_t head_elem(int32_t dtype) { return dtype == ETS_DTYPE_FLOAT ? 4 : 2; }
+bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// Workgroups for `count` elements, one per lane, a few rounds at most.
+uint32_t layout_grid(int64_t count) {
+  return static_cast<uint32_t>(std::min<int64_t>((count + ets::kHeadBlock - 1) / ets::kHeadBlock, 1 << 20));
+}
+
+}  // namespace
+
+extern "C" {
+
+ets_status ets_logit_head_create(int32_t vocab_size, int32_t hidden_size, int32_t group_size, const void* d_packed,
+                                 int64_t packed_stride, const void* d_scales, const void* d_zeros, int32_t scale_dtype,
+                                 void* hip_stream, ets_logit_head** out) {
+  if (!out) return head_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_logit_head_create: out is null");
+  *out = nullptr;
+  if (vocab_size < 1 || hidden_size < 1)
+    return head_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_logit_head_create: vocab_size and hidden_size must be >= 1");
+  if (vocab_size >= (1 << 24) || hidden_size > (1 << 20))
+    return head_fail(nullptr, ETS_NOT_SUPPORTED, "ets_logit_head_create: vocab_size must be below 16777216, hidden_size at most 1048576");
+  if (group_size != 32 && group_size != 64 && (group_size < 128 || group_size % 128 != 0))
+    return head_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_logit_head_create: group_size must be 32, 64 or a multiple of 128");
+  if (!head_dtype(scale_dtype))
+    return head_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_logit_head_create: scale type must be Float, Half or BFloat16");
+  if (!d_packed || !d_scales) return head_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_logit_head_create: null pointer");
+  if (packed_stride < (hidden_size + 1) / 2)
+    return head_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_logit_head_create: packed rows shorter than hidden_size");
+  const size_t scale_bytes = head_elem(scale_dtype);
+  if (!aligned_to(d_scales, scale_bytes) || !aligned_to(d_zeros, scale_bytes))
+    return head_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_logit_head_create: pointer not aligned to its element type");
+  ets_logit_head* h = new (std::nothrow) ets_logit_head();
+  if (!h) return head_fail(nullptr, ETS_MEMORY_ALLOCATION_FAILED, "ets_logit_head_create: out of host memory");
+  h->vocab = vocab_size;
+  h->hidden = hidden_size;
+  h->tiles = (vocab_size + ets::kTileRows - 1) / ets::kTileRows;
+  h->chunks = (hidden_size + ets::kChunkCols - 1) / ets::kChunkCols;
+  h->form.groups_per_chunk = group_size < ets::kChunkCols ? ets::kChunkCols / group_size : 1;
+  h->form.scale_bytes = static_cast<int>(scale_bytes);
+  h->form.zeros = d_zeros != nullptr;
+  h->scale_is_bf16 = scale_dtype == ETS_DTYPE_BFLOAT16;
+  h->chunks_per_group = group_size < ets::kChunkCols ? 1 : std::min(group_size / ets::kChunkCols, h->chunks);
+  const int32_t groups = (hidden_size - 1) / group_size + 1;  // of a row, as the caller has them
+  h->groups = groups;
+  auto bail = [&](hipError_t e, const char* what) {
+    const ets_status st = head_hip_fail(nullptr, e, what);
+    ets_logit_head_destroy(h);
+    return st;
+  };
+  hipError_t e = hipGetDevice(&h->device);
+  if (e != hipSuccess) return bail(e, "ets_logit_head_create: hipGetDevice");
+  hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+  const int64_t dwords = static_cast<int64_t>(h->tiles) * h->chunks * 256;
+  e = hipMalloc(&h->d_blocks, dwords * 4);
+  if (e != hipSuccess) return bail(e, "ets_logit_head_create: hipMalloc(weights)");
+  hipLaunchKernelGGL(ets::head_layout_kernel, dim3(layout_grid(dwords)), dim3(ets::kHeadBlock), 0, stream,
+                     static_cast<const uint8_t*>(d_packed), packed_stride, vocab_size, hidden_size, h->chunks, dwords,
+                     static_cast<uint32_t*>(h->d_blocks));
+  e = hipGetLastError();
+  if (e != hipSuccess) return bail(e, "ets_logit_head_create: launch");
+  const int32_t per_chunk = h->form.groups_per_chunk;
+  const int64_t per_tile = static_cast<int64_t>(ets::kTileRows) * (per_chunk > 1 ? h->chunks * per_chunk : groups);
+  const int64_t count = per_tile * h->tiles;
+  for (int k = 0; k < (d_zeros ? 2 : 1); ++k) {
+    void** dst = k ? &h->d_zeros : &h->d_scales;
+    const void* src = k ? d_zeros : d_scales;
+    e = hipMalloc(dst, count * scale_bytes);
+    if (e != hipSuccess) return bail(e, "ets_logit_head_create: hipMalloc(scales)");
+    if (scale_bytes == 4) {
+      hipLaunchKernelGGL((ets::head_scales_kernel<uint32_t>), dim3(layout_grid(count)), dim3(ets::kHeadBlock), 0, stream,
+                         static_cast<const uint32_t*>(src), vocab_size, groups, per_chunk, per_tile, count, static_cast<uint32_t*>(*dst));
+    } else {
+      hipLaunchKernelGGL((ets::head_scales_kernel<uint16_t>), dim3(layout_grid(count)), dim3(ets::kHeadBlock), 0, stream,
+                         static_cast<const uint16_t*>(src), vocab_size, groups, per_chunk, per_tile, count, static_cast<uint16_t*>(*dst));
+    }
+    e = hipGetLastError();
+    if (e != hipSuccess) return bail(e, "ets_logit_head_create: launch");
+  }
+  e = hipStreamSynchronize(stream);
+  if (e != hipSuccess) return bail(e, "ets_logit_head_create: hipStreamSynchronize");
+  *out = h;
+  return ETS_OK;
+}
+
+ets_status ets_logit_head_destroy(ets_logit_head* h) {
+  if (!h) return ETS_OK;
+  {
+    ets_host::DeviceGuard g(h->device);
+    (void)hipFree(h->d_blocks);
+    (void)hipFree(h->d_scales);
+    (void)hipFree(h->d_zeros);
+  }
+  delete h;
+  return ETS_OK;
+}
+
+ets_status ets_logit_head_logits(ets_logit_head* h, const void* d_hidden, int32_t dtype, int32_t rows, int64_t hidden_stride,
+                                 void* d_logits, int32_t logits_dtype, int64_t logits_stride, void* hip_stream) {
+  if (!h) return head_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_logit_head_logits: null handle");
+  h->last_error[0] = 0;
+  if (!head_dtype(dtype) || !head_dtype(logits_dtype))
+    return head_fail(h, ETS_INVALID_ARGUMENT, "ets_logit_head_logits: element types must be Float, Half or BFloat16");
+  if (rows < 0) return head_fail(h, ETS_INVALID_ARGUMENT, "ets_logit_head_logits: rows must be >= 0");
+  if (rows > 65535 * 16) return head_fail(h, ETS_NOT_SUPPORTED, "ets_logit_head_logits: at most 1048560 rows in one call");
+  if (rows == 0) return ETS_OK;
+  if (!d_hidden || !d_logits) return head_fail(h, ETS_INVALID_ARGUMENT, "ets_logit_head_logits: null pointer");
+  if (rows > 1 && (hidden_stride < h->hidden || logits_stride < h->vocab))
+    return head_fail(h, ETS_INVALID_ARGUMENT, "ets_logit_head_logits: row stride smaller than the row");
+  if (!aligned_to(d_hidden, head_elem(dtype)) || !aligned_to(d_logits, head_elem(logits_dtype)))
+    return head_fail(h, ETS_INVALID_ARGUMENT, "ets_logit_head_logits: pointer not aligned to its element type");
+  ets::HeadParams p = {};
+  p.blocks = static_cast<const ets::u32x4*>(h->d_blocks);
+  p.scales = h->d_scales;
+  p.zeros = h->d_zeros;
+  p.scale_is_bf16 = h->scale_is_bf16;
+  p.tiles = h->tiles;
+  p.chunks = h->chunks;
+  p.chunks_per_group = h->chunks_per_group;
+  p.groups = h->groups;
+  p.vocab = h->vocab;
+  p.hidden = h->hidden;
+  p.rows = rows;
+  p.x = d_hidden;
+  p.x_stride = hidden_stride;
+  p.out = d_logits;
+  p.out_stride = logits_stride;
+  p.out_dtype = logits_dtype;
+  ets_host::DeviceGuard g(h->device);
+  hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+  hipError_t e = hipSuccess;
+  switch (dtype) {
+    case ETS_DTYPE_FLOAT: e = ets_host::launch_head_f32(p, h->form, stream); break;
+    case ETS_DTYPE_HALF: e = ets_host::launch_head_f16(p, h->form, stream); break;
+    default: e = ets_host::launch_head_bf16(p, h->form, stream); break;
+  }
+  return e == hipSuccess ? ETS_OK : head_hip_fail(h, e, "ets_logit_head_logits: launch");
+}
+
+ets_status ets_sampler_sample_hidden(ets_sampler* s, ets_logit_head* h, const void* d_hidden, int32_t dtype, int32_t rows,
+                                     int64_t hidden_stride, void* d_logits, int32_t logits_dtype, int64_t logits_stride,
+                                     int32_t* d_tokens, void* hip_stream) {
+  using ets_host::fail;
+  if (!s) return fail(nullptr, ETS_INVALID_ARGUMENT, "ets_sampler_sample_hidden: null handle");
+  s->last_error.clear();
+  if (!h) return fail(s, ETS_INVALID_ARGUMENT, "ets_sampler_sample_hidden: null head");
+  if (h->vocab != s->vocab) return fail(s, ETS_INVALID_ARGUMENT, "ets_sampler_sample_hidden: the head's vocabulary is not the sampler's");
+  if (h->device != s->device) return fail(s, ETS_INVALID_ARGUMENT, "ets_sampler_sample_hidden: head and sampler live on different devices");
+  // (what the sampler would refuse is refused before the logits are written)
+  if (rows < 0 || rows > s->max_batch)
+    return fail(s, ETS_INVALID_ARGUMENT, "ets_sampler_sample_hidden: rows exceeds the sampler's max_batch");
+  if (rows == 0) return ETS_OK;
+  if (!d_tokens) return fail(s, ETS_INVALID_ARGUMENT, "ets_sampler_sample_hidden: null pointer");
+  if (logits_stride < s->vocab)
+    return fail(s, ETS_INVALID_ARGUMENT, "ets_sampler_sample_hidden: logits row stride smaller than vocab_size");
+  ets_status st = ets_logit_head_logits(h, d_hidden, dtype, rows, hidden_stride, d_logits, logits_dtype, logits_stride, hip_stream);
+  if (st != ETS_OK) return fail(s, st, h->last_error);
+  return ets_sampler_sample_batch(s, d_logits, logits_dtype, rows, logits_stride, d_tokens, hip_stream);
+}
+
+const char* ets_logit_head_last_error(const ets_logit_head* h) { return h ? h->last_error : g_head_error; }
+
+}  // extern "C"

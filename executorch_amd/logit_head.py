@@ -1,0 +1,79 @@
+"""The logits head with 4-bit weights over the C ABI of include/et_logit_head.h.
+
+``LogitHead(packed, scales, group_size)`` lays a ``[vocab, hidden]`` matrix of 4-bit weights with group
+scales out once; :meth:`LogitHead.logits` multiplies hidden states with it.
+:meth:`executorch_amd.Sampler.sample_hidden` goes from hidden states to tokens.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _capi
+from .sampler import SamplerError, dtype_code
+
+
+class LogitHead:
+    """``packed``: uint8 ``[vocab, (hidden + 1) // 2]``, column 2j in the low nibble of byte j, 2j + 1 in the
+    high one; ``scales`` (and ``zeros``): ``[vocab, ceil(hidden / group_size)]``, fp32, fp16 or bf16; a
+    weight is ``(nibble - 8) * scale + zero`` of its group.  ``group_size``: 32, 64 or a multiple of 128.
+    The tensors are copied into a layout of the head's own and may be freed afterwards."""
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, group_size: int, hidden_size: int | None = None,
+                 zeros: torch.Tensor | None = None):
+        self._h = C.c_void_p()
+        if packed.dim() != 2 or packed.dtype != torch.uint8 or not packed.is_cuda or (packed.stride(1) != 1 and packed.shape[1] > 1):
+            raise SamplerError(_capi.INVALID_ARGUMENT, "packed must be a uint8 device tensor [vocab, (hidden + 1) // 2] with unit inner stride")
+        vocab, width = packed.shape
+        hidden = 2 * width if hidden_size is None else int(hidden_size)
+        if hidden < 1 or (hidden + 1) // 2 != width:
+            raise SamplerError(_capi.INVALID_ARGUMENT, "packed must have (hidden_size + 1) // 2 columns")
+        if group_size < 1:
+            raise SamplerError(_capi.INVALID_ARGUMENT, "group_size must be 32, 64 or a multiple of 128")
+        shape = (vocab, (hidden + group_size - 1) // group_size)
+        for t, name in ((scales, "scales"), (zeros, "zeros")):
+            if t is not None and not (t.device == packed.device and t.shape == shape and t.is_contiguous() and t.dtype == scales.dtype):
+                raise SamplerError(_capi.INVALID_ARGUMENT, f"{name} must be a contiguous tensor {list(shape)} next to packed, scales and zeros of one type")
+        self.device = packed.device
+        with torch.cuda.device(self.device):
+            st = _capi.lib().ets_logit_head_create(
+                vocab, hidden, group_size, packed.data_ptr(), packed.stride(0), scales.data_ptr(),
+                zeros.data_ptr() if zeros is not None else None, dtype_code(scales),
+                torch.cuda.current_stream(self.device).cuda_stream, C.byref(self._h))
+        if st != _capi.OK:
+            raise SamplerError(st, _capi.lib().ets_logit_head_last_error(None).decode())
+        self.vocab_size, self.hidden_size, self.group_size = vocab, hidden, group_size
+
+    def close(self) -> None:
+        if getattr(self, "_h", None) and self._h.value:
+            _capi.lib().ets_logit_head_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def logits(self, hidden: torch.Tensor, out: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """``hidden`` ``[rows, hidden]`` (fp32, fp16 or bf16, unit inner stride) -> ``[rows, vocab]`` of ``dtype``
+        (default: that of ``out``, or of ``hidden``), asynchronously on the current stream."""
+        out = self._output(hidden, out, dtype)
+        st = _capi.lib().ets_logit_head_logits(self._h, hidden.data_ptr(), dtype_code(hidden), hidden.shape[0], hidden.stride(0),
+                                               out.data_ptr(), dtype_code(out), out.stride(0),
+                                               torch.cuda.current_stream(self.device).cuda_stream)
+        if st != _capi.OK:
+            raise SamplerError(st, _capi.lib().ets_logit_head_last_error(self._h).decode())
+        return out
+
+    def _output(self, hidden, out, dtype) -> torch.Tensor:
+        if hidden.device != self.device or hidden.dim() != 2 or hidden.shape[1] != self.hidden_size or \
+                (hidden.stride(1) != 1 and self.hidden_size > 1):
+            raise SamplerError(_capi.INVALID_ARGUMENT, f"hidden must be [rows, {self.hidden_size}] on {self.device} with unit inner stride")
+        if out is None:
+            return torch.empty((hidden.shape[0], self.vocab_size), dtype=dtype or hidden.dtype, device=self.device)
+        if out.device != self.device or out.shape != (hidden.shape[0], self.vocab_size) or (out.stride(1) != 1 and self.vocab_size > 1) or \
+                (dtype is not None and out.dtype != dtype):
+            raise SamplerError(_capi.INVALID_ARGUMENT, f"out must be [rows, {self.vocab_size}] on {self.device} with unit inner stride")
+        return out

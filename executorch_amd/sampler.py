@@ -207,6 +207,21 @@ class Sampler:
             self._h, chain._h, logits.data_ptr(), code, B, logits.stride(0), out.data_ptr(), stream))
         return out
 
+    def sample_hidden(self, hidden: torch.Tensor, head, logits: torch.Tensor | None = None, dtype: torch.dtype | None = None,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+        """Hidden states ``[B, hidden]`` to tokens: ``head.logits(hidden, out=logits, dtype=dtype)`` followed by
+        ``sample_batch`` of them, in one call.  Pass ``logits`` to keep them."""
+        logits = head._output(hidden, logits, dtype)
+        if out is None:
+            out = torch.empty(hidden.shape[0], dtype=torch.int32, device=hidden.device)
+        stream = torch.cuda.current_stream(hidden.device).cuda_stream
+        # (a tensor of one row may have any stride; the call wants one that holds the row)
+        self._check(_capi.lib().ets_sampler_sample_hidden(
+            self._h, head._h, hidden.data_ptr(), dtype_code(hidden), hidden.shape[0], hidden.stride(0), logits.data_ptr(),
+            dtype_code(logits), max(logits.stride(0), logits.shape[1]) if logits.shape[0] <= 1 else logits.stride(0),
+            out.data_ptr(), stream))
+        return out
+
     def gumbel_max_batch(self, logits: torch.Tensor, temperature, noise: torch.Tensor | None = None,
                          out: torch.Tensor | None = None, dtype: int | None = None) -> torch.Tensor:
         """The in-graph Gumbel-max sampler (examples/models/qwen3_5_moe/sampler.py:17-60):

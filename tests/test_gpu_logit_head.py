@@ -1,0 +1,244 @@
+"""LogitHead through the C ABI against the float64 restatement, within the bound derived there."""
+import numpy as np
+import pytest
+import torch
+
+import executorch_amd as ea
+from executorch_amd import _capi
+from oracle import head_oracle as HO
+from oracle import verify_oracle as VO
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def weights(seed, vocab, hidden, group, scale_dtype, zeros, dev):
+    g = np.random.default_rng(seed)
+    groups = -(-hidden // group)
+    packed = torch.from_numpy(g.integers(0, 256, size=(vocab, (hidden + 1) // 2), dtype=np.uint8)).to(dev)
+    scales = torch.from_numpy((0.02 * (g.random((vocab, groups)) - 0.3)).astype(np.float32)).to(dev).to(DT[scale_dtype])
+    z = torch.from_numpy((0.05 * g.standard_normal((vocab, groups))).astype(np.float32)).to(dev).to(DT[scale_dtype]) if zeros else None
+    return packed, scales, z
+
+
+def states(seed, rows, hidden, dtype, dev):
+    g = np.random.default_rng(seed + 1000)
+    x = g.standard_normal((rows, hidden)).astype(np.float32)
+    x[:, g.integers(0, hidden, size=1)] *= 30
+    return torch.from_numpy(x).to(dev).to(DT[dtype])
+
+
+def host(t):
+    return None if t is None else t.float().cpu().numpy()
+
+
+def check(y, x, w, group, out_dtype, label):
+    packed, scales, zeros = w
+    want, bound = HO.logits(host(x), packed.cpu().numpy(), host(scales), host(zeros), group, out_dtype)
+    got = y.double().cpu().numpy()
+    off = np.abs(got - want)
+    worst = np.unravel_index(np.argmax(off - bound), off.shape)
+    assert (off <= bound).all(), (label, worst, got[worst], want[worst], bound[worst])
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f16", "f32"), ("f32", "f32"), ("f32", "bf16"), ("bf16", "f16")])
+@pytest.mark.parametrize("group", [32, 64, 128, 256, 384, 1 << 20])
+@pytest.mark.parametrize("scale_dtype,zeros", [("bf16", False), ("f16", True), ("f32", False), ("f32", True), ("bf16", True)])
+def test_types_and_groups(dev, dtype, out_dtype, group, scale_dtype, zeros):
+    rows, vocab, hidden = 5, 130, 1000
+    w = weights(group + 7, vocab, hidden, group, scale_dtype, zeros, dev)
+    x = states(group, rows, hidden, dtype, dev)
+    head = ea.LogitHead(w[0], w[1], group, zeros=w[2])
+    check(head.logits(x, dtype=DT[out_dtype]), x, w, group, out_dtype, (dtype, out_dtype, group))
+
+
+@pytest.mark.parametrize("vocab", [1, 15, 16, 17, 63, 64, 65, 1000])
+@pytest.mark.parametrize("hidden", [1, 2, 31, 33, 127, 128, 129, 256, 777])
+def test_odd_sizes(dev, vocab, hidden):
+    for rows, dtype, group in ((1, "bf16", 32), (3, "f32", 64), (17, "f16", 128)):
+        w = weights(vocab * 3 + hidden, vocab, hidden, group, "f32", True, dev)
+        x = states(hidden, rows, hidden, dtype, dev)
+        head = ea.LogitHead(w[0], w[1], group, hidden_size=hidden, zeros=w[2])
+        check(head.logits(x, dtype=torch.float32), x, w, group, "f32", (vocab, hidden, rows))
+
+
+@pytest.mark.parametrize("dtype,group,zeros", [("bf16", 128, False), ("bf16", 32, True), ("f16", 64, False), ("f16", 32, False), ("f32", 32, False), ("f32", 256, True)])
+def test_every_number_of_rows(dev, dtype, group, zeros):
+    vocab, hidden = 515, 640
+    w = weights(5, vocab, hidden, group, "f32" if dtype == "f32" else dtype, zeros, dev)
+    head = ea.LogitHead(w[0], w[1], group, zeros=w[2])
+    for rows in (1, 2, 4, 7, 8, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65, 96, 127, 128, 129, 160, 200, 320, 513):
+        x = states(rows, rows, hidden, dtype, dev)
+        check(head.logits(x, dtype=torch.float32), x, w, group, "f32", (dtype, group, rows))
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,group,dtype", [(1, 128256, 512, 128, "bf16"), (6, 32000, 2048, 32, "f16"), (64, 20000, 1024, 128, "bf16"),
+                                                            (130, 9000, 2050, 64, "bf16"), (320, 5000, 1536, 128, "bf16")])
+def test_larger(dev, rows, vocab, hidden, group, dtype):
+    w = weights(11, vocab, hidden, group, dtype, False, dev)
+    x = states(3, rows, hidden, dtype, dev)
+    head = ea.LogitHead(w[0], w[1], group)
+    check(head.logits(x), x, w, group, dtype, (rows, vocab, hidden))
+
+
+def test_wide_values(dev):
+    """fp32 hidden states over many binades (the three bf16 parts hold all of their bits) and fp16 ones at both ends."""
+    vocab, hidden, group = 80, 500, 32
+    w = weights(21, vocab, hidden, group, "f32", True, dev)
+    head = ea.LogitHead(w[0], w[1], group, zeros=w[2])
+    g = np.random.default_rng(2)
+    x = torch.from_numpy((g.standard_normal((9, hidden)) * 2.0 ** g.integers(-60, 60, size=(9, hidden))).astype(np.float32)).to(dev)
+    check(head.logits(x), x, w, group, "f32", "wide")
+    x = torch.from_numpy((g.standard_normal((9, hidden)) * 2.0 ** g.integers(-20, 12, size=(9, hidden))).astype(np.float16)).to(dev)
+    check(head.logits(x, dtype=torch.float32), x, w, group, "f32", "fp16")
+    # one column at a time gives the weight itself, scaled
+    eye = torch.eye(hidden, device=dev)
+    check(head.logits(eye), eye, w, group, "f32", "columns")
+
+
+@pytest.mark.parametrize("rows", [1, 20, 100])
+def test_strides_gaps_and_what_lies_beside(dev, rows):
+    vocab, hidden, group = 203, 301, 64
+    w = weights(31, vocab, hidden, group, "bf16", False, dev)
+    wide = torch.full((vocab, w[0].shape[1] + 5), 255, dtype=torch.uint8, device=dev)
+    wide[:, :-5] = w[0]
+    head = ea.LogitHead(wide[:, :-5], w[1], group, hidden_size=hidden)
+    wide.zero_()  # (the head has its own copy)
+    for dtype in ("bf16", "f32"):
+        x = states(7, rows, hidden, dtype, dev)
+        spread = torch.full((rows + 2, hidden + 3), float("nan"), dtype=DT[dtype], device=dev)
+        spread[1:-1, 1:hidden + 1] = x  # rows that start at odd elements, NaN around them
+        out = torch.full((rows + 2, vocab + 7), 5.0, dtype=torch.float32, device=dev)
+        y = head.logits(spread[1:-1, 1:hidden + 1], out=out[1:-1, 3:vocab + 3])
+        check(y, x, w, group, "f32", (rows, dtype))
+        assert (out[0] == 5).all() and (out[-1] == 5).all() and (out[:, :3] == 5).all() and (out[:, vocab + 3:] == 5).all()
+
+
+def test_logits_further_than_31_bits_apart(dev):
+    vocab, hidden, group, rows = 100, 128, 128, 3
+    w = weights(41, vocab, hidden, group, "bf16", False, dev)
+    x = states(9, rows, hidden, "bf16", dev)
+    far = (1 << 30) + 77
+    flat = torch.zeros((rows - 1) * far + vocab, dtype=torch.bfloat16, device=dev)
+    out = flat.as_strided((rows, vocab), (far, 1))
+    check(ea.LogitHead(w[0], w[1], group).logits(x, out=out), x, w, group, "bf16", "far")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_rows_that_are_not_finite_stay_to_themselves(dev, dtype):
+    vocab, hidden, group = 70, 256, 32
+    w = weights(51, vocab, hidden, group, "f32", False, dev)
+    head = ea.LogitHead(w[0], w[1], group)
+    for rows in (4, 40):
+        x = states(1, rows, hidden, dtype, dev)
+        good = head.logits(x, dtype=torch.float32)
+        x[1, 3], x[2, 200] = float("nan"), float("inf")
+        y = head.logits(x, dtype=torch.float32)
+        assert not torch.isfinite(y[1]).any() and not torch.isfinite(y[2]).any()
+        keep = [r for r in range(rows) if r not in (1, 2)]
+        assert torch.equal(y[keep], good[keep])
+
+
+def test_no_rows(dev):
+    w = weights(61, 64, 128, 128, "f32", False, dev)
+    y = ea.LogitHead(w[0], w[1], 128).logits(torch.zeros((0, 128), device=dev))
+    assert y.shape == (0, 64)
+
+
+def test_streams_and_graphs(dev):
+    """One head on two streams at once, and captured: replays see the present hidden states."""
+    vocab, hidden, group = 4000, 1024, 128
+    w = weights(71, vocab, hidden, group, "bf16", False, dev)
+    head = ea.LogitHead(w[0], w[1], group)
+    xs = [states(s, rows, hidden, "bf16", dev) for s, rows in ((1, 3), (2, 90))]
+    want = [head.logits(x) for x in xs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((head.logits(xs[k]), want[k]))
+    torch.cuda.synchronize()
+    for a, b in got:
+        assert torch.equal(a, b)
+    for k, x in enumerate(xs):
+        out = torch.empty_like(want[k])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            head.logits(x, out=out)
+        for r in range(3):
+            x.copy_(states(100 + r, x.shape[0], hidden, "bf16", dev))
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, head.logits(x))
+            check(out, x, w, group, "bf16", ("replay", k, r))
+
+
+def test_hidden_states_to_tokens(dev):
+    vocab, hidden, group, rows = 32000, 512, 64, 9
+    w = weights(81, vocab, hidden, group, "bf16", False, dev)
+    head = ea.LogitHead(w[0], w[1], group)
+    one, two = (ea.Sampler(vocab, 0.7, 0.9, 4, max_batch=rows) for _ in range(2))
+    for step in range(3):
+        x = states(step, rows, hidden, "bf16", dev)
+        logits = torch.empty((rows, vocab), dtype=torch.bfloat16, device=dev)
+        tokens = one.sample_hidden(x, head, logits=logits)
+        want = head.logits(x)
+        assert torch.equal(logits, want) and torch.equal(tokens, two.sample_batch(want))
+        assert np.array_equal(one.get_rng_states(), two.get_rng_states())
+    assert torch.equal(one.sample_hidden(x[:1], head, dtype=torch.float32), two.sample_batch(head.logits(x[:1], dtype=torch.float32)))
+    assert one.sample_hidden(x[:0], head).shape == (0,)
+    before = one.get_rng_states()
+    other = ea.Sampler(vocab + 1, 0.7, 0.9, 4, max_batch=rows)
+    for bad in (lambda: other.sample_hidden(x, head), lambda: ea.Sampler(vocab, 0.7, 0.9, 4, max_batch=2).sample_hidden(x, head),
+                lambda: one.sample_hidden(x[:, :-1], head), lambda: one.sample_hidden(x, head, logits=logits[:, :-1])):
+        with pytest.raises(ea.SamplerError):
+            bad()
+    assert np.array_equal(one.get_rng_states(), before)
+
+
+def test_a_speculative_step(dev):
+    """The operators as they are used together: a draft head proposes through the sampler, the target head
+    scores all positions at once, the verifier decides; its answer is the float64 restatement's over the
+    logits that the heads made."""
+    S, K, vocab, hidden = 5, 3, 5000, 256
+    target_w, draft_w = weights(91, vocab, hidden, 64, "bf16", False, dev), weights(91, vocab, hidden, 128, "bf16", False, dev)
+    target, draft = ea.LogitHead(target_w[0], target_w[1], 64), ea.LogitHead(draft_w[0], draft_w[1], 128)
+    temperature = 0.8
+    smp = ea.Sampler(vocab, temperature, 1.0, 12, max_batch=S)
+    v = ea.DraftVerifier(vocab, S, K)
+    for step in range(4):
+        x = states(200 + step, S * (K + 1), hidden, "bf16", dev).view(S, K + 1, hidden)
+        draft_logits = torch.empty((S, K, vocab), dtype=torch.bfloat16, device=dev)
+        tokens = torch.empty((S, K), dtype=torch.int32, device=dev)
+        for i in range(K):
+            step_logits = torch.empty((S, vocab), dtype=torch.bfloat16, device=dev)
+            tokens[:, i] = smp.sample_hidden(x[:, i], draft, logits=step_logits)
+            draft_logits[:, i] = step_logits
+        target_logits = target.logits(x.reshape(-1, hidden)).view(S, K + 1, vocab)
+        coins = torch.rand((S, K + 1), device=dev)
+        got, accepted = v.verify(target_logits, tokens, coins, draft_logits=draft_logits, temperature=temperature)
+        want, n = VO.verify(host(target_logits), host(draft_logits), tokens.cpu().numpy(), None, [np.float32(temperature)] * S, coins.cpu().numpy())
+        assert np.array_equal(got.cpu().numpy(), want) and np.array_equal(accepted.cpu().numpy(), n)
+
+
+def test_refusals(dev):
+    w = weights(1, 64, 256, 128, "bf16", False, dev)
+    head = ea.LogitHead(w[0], w[1], 128)
+    x = states(1, 2, 256, "bf16", dev)
+    for bad in (lambda: head.logits(x[:, :-1]), lambda: head.logits(x[0]), lambda: head.logits(x.cpu()), lambda: head.logits(x.double()),
+                lambda: head.logits(x.t().contiguous().t()), lambda: head.logits(x, out=torch.zeros((2, 63), device=dev)),
+                lambda: head.logits(x, out=torch.zeros((2, 64), device=dev), dtype=torch.bfloat16),
+                lambda: head.logits(x, out=torch.zeros((64, 2), device=dev).t()), lambda: head.logits(x, dtype=torch.float64),
+                lambda: head.logits(x, out=torch.zeros((1, 64), device=dev).expand(2, 64)),
+                lambda: ea.LogitHead(w[0].int(), w[1], 128), lambda: ea.LogitHead(w[0], w[1], 64), lambda: ea.LogitHead(w[0], w[1].cpu(), 128),
+                lambda: ea.LogitHead(w[0], w[1].double(), 128), lambda: ea.LogitHead(w[0], w[1], 128, hidden_size=258),
+                lambda: ea.LogitHead(w[0], w[1], 128, zeros=w[1].float()), lambda: ea.LogitHead(w[0], w[1], 0),
+                lambda: ea.LogitHead(w[0], w[1][:, :0].contiguous(), 96)):
+        with pytest.raises(ea.SamplerError) as e:
+            bad()
+        assert e.value.code == _capi.INVALID_ARGUMENT
+    check(head.logits(x), x, w, 128, "bf16", "the head still works")
