@@ -1,6 +1,7 @@
 // Host side of include/et_speculative.h: the verification of drafted tokens.
 #include "../../include/et_speculative.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <new>
@@ -10,9 +11,11 @@
 
 struct ets_verifier {
   int32_t vocab = 0, max_sequences = 0, max_drafts = 0;
-  int device = 0;
-  ets::ChunkStat* d_stats = nullptr;  // [max_sequences, 2 max_drafts + 1, chunks of kSmallChunk]
-  double* d_rest = nullptr;           // [max_sequences, chunks of kSmallChunk]
+  int device = 0, num_cus = 0;
+  ets::ChunkStat* d_stats = nullptr;  // [max_sequences, 2 max_drafts + 1, chunks]
+  ets::ChunkMass* d_mass = nullptr;   // [max_sequences, chunks]
+  ets::Decision* d_decisions = nullptr;  // [max_sequences]
+  float* d_token_logits = nullptr;    // [max_sequences, 2 max_drafts + 1]
   double* d_exp2 = nullptr;           // 2^(j / kExp2Steps)
   char last_error[256] = "";
 };
@@ -30,38 +33,31 @@ ets_status verifier_hip_fail(ets_verifier* v, hipError_t e, const char* what) {
   return verifier_fail(v, e == hipErrorOutOfMemory ? ETS_MEMORY_ALLOCATION_FAILED : ETS_INTERNAL, what, hipGetErrorString(e));
 }
 
-int64_t chunks_of(int32_t vocab, int32_t chunk) { return (static_cast<int64_t>(vocab) + chunk - 1) / chunk; }
+int32_t chunks_of(int32_t vocab) { return (vocab + ets::kVerifyChunk - 1) / ets::kVerifyChunk; }
 
 bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-template <int DT, int CHUNK>
-hipError_t launch_verify(const ets::VerifyParams& p, hipStream_t stream) {
-  constexpr int U = CHUNK / (ets::kVerifyBlock * ets::VecElems<DT>::value);
-  const int64_t rows = static_cast<int64_t>(p.sequences) * p.rows_per_seq;
-  hipLaunchKernelGGL((ets::verify_stats_kernel<DT, U>), dim3(static_cast<uint32_t>(rows * p.chunks)), dim3(ets::kVerifyBlock), 0,
-                     stream, p);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  if (p.draft) {
-    hipLaunchKernelGGL((ets::verify_rest_kernel<DT, U>), dim3(static_cast<uint32_t>(static_cast<int64_t>(p.sequences) * p.chunks)),
-                       dim3(ets::kVerifyBlock), 0, stream, p);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  hipLaunchKernelGGL((ets::verify_finish_kernel<DT, CHUNK>), dim3(p.sequences), dim3(ets::kFinishBlock), 0, stream, p);
-  return hipGetLastError();
-}
-
 template <int DT>
-hipError_t launch_verify(ets::VerifyParams p, hipStream_t stream) {
-  // Large chunks when there are enough of them to fill the chip twice over, small ones otherwise.
-  const int64_t rows = static_cast<int64_t>(p.sequences) * p.rows_per_seq;
-  if (rows * chunks_of(p.vocab, ets::kLargeChunk) >= 512) {
-    p.chunks = static_cast<int32_t>(chunks_of(p.vocab, ets::kLargeChunk));
-    return launch_verify<DT, ets::kLargeChunk>(p, stream);
+hipError_t launch_verify(ets::VerifyParams p, int num_cus, hipStream_t stream) {
+  constexpr int kWaves = ets::kVerifyWaves;
+  // Statistics: as many workgroups as are resident at once, each wave taking several chunks.
+  const int64_t items = static_cast<int64_t>(p.sequences) * p.rows_per_seq * p.chunks;
+  const int64_t groups = std::min<int64_t>((items + kWaves - 1) / kWaves, (DT == ets::kDtypeFloat ? 5 : 7) * num_cus);
+  const int64_t stride = groups * kWaves;
+  p.step_chunk = static_cast<int32_t>(stride % p.chunks);
+  p.step_j = static_cast<int32_t>(stride / p.chunks % p.rows_per_seq);
+  p.step_b = static_cast<int32_t>(stride / p.chunks / p.rows_per_seq);
+  hipLaunchKernelGGL((ets::verify_stats_kernel<DT>), dim3(static_cast<uint32_t>(groups)), dim3(ets::kVerifyBlock), 0, stream, p);
+  // With up to two workgroups per CU in verify_rest the decision costs less inside it than a launch would.
+  const int64_t chunks = static_cast<int64_t>(p.sequences) * p.chunks;
+  if (chunks > 2 * num_cus) {
+    hipLaunchKernelGGL((ets::verify_decide_kernel<DT>), dim3(p.sequences), dim3(ets::kVerifyBlock), 0, stream, p);
+    hipLaunchKernelGGL((ets::verify_rest_kernel<DT, true>), dim3(static_cast<uint32_t>(chunks)), dim3(ets::kVerifyBlock), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL((ets::verify_rest_kernel<DT, false>), dim3(static_cast<uint32_t>(chunks)), dim3(ets::kVerifyBlock), 0, stream, p);
   }
-  p.chunks = static_cast<int32_t>(chunks_of(p.vocab, ets::kSmallChunk));
-  return launch_verify<DT, ets::kSmallChunk>(p, stream);
+  hipLaunchKernelGGL((ets::verify_finish_kernel<DT>), dim3(p.sequences), dim3(ets::kVerifyBlock), 0, stream, p);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -76,7 +72,7 @@ ets_status ets_verifier_create(int32_t vocab_size, int32_t max_sequences, int32_
   if (max_sequences < 1) return verifier_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_verifier_create: max_sequences must be >= 1");
   if (max_drafts < 0) return verifier_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_verifier_create: max_drafts must be >= 0");
   if (max_drafts > ets::kMaxDrafts) return verifier_fail(nullptr, ETS_NOT_SUPPORTED, "ets_verifier_create: max_drafts must be at most 64");
-  const int64_t chunks = chunks_of(vocab_size, ets::kSmallChunk);
+  const int64_t chunks = chunks_of(vocab_size);
   if (max_sequences > 65535 || static_cast<int64_t>(max_sequences) * (2 * max_drafts + 1) * chunks > INT32_MAX)
     return verifier_fail(nullptr, ETS_NOT_SUPPORTED, "ets_verifier_create: max_sequences x max_drafts x vocab_size is too large for one launch");
   ets_verifier* v = new (std::nothrow) ets_verifier();
@@ -91,11 +87,17 @@ ets_status ets_verifier_create(int32_t vocab_size, int32_t max_sequences, int32_
   };
   hipError_t e = hipGetDevice(&v->device);
   if (e != hipSuccess) return bail(e, "ets_verifier_create: hipGetDevice");
+  e = hipDeviceGetAttribute(&v->num_cus, hipDeviceAttributeMultiprocessorCount, v->device);
+  if (e != hipSuccess) return bail(e, "ets_verifier_create: hipDeviceGetAttribute(MultiprocessorCount)");
   const size_t rows = static_cast<size_t>(max_sequences) * (2 * max_drafts + 1);
   e = hipMalloc(reinterpret_cast<void**>(&v->d_stats), rows * chunks * sizeof(ets::ChunkStat));
   if (e != hipSuccess) return bail(e, "ets_verifier_create: hipMalloc(statistics)");
-  e = hipMalloc(reinterpret_cast<void**>(&v->d_rest), static_cast<size_t>(max_sequences) * chunks * sizeof(double));
-  if (e != hipSuccess) return bail(e, "ets_verifier_create: hipMalloc(residual masses)");
+  e = hipMalloc(reinterpret_cast<void**>(&v->d_mass), static_cast<size_t>(max_sequences) * chunks * sizeof(ets::ChunkMass));
+  if (e != hipSuccess) return bail(e, "ets_verifier_create: hipMalloc(masses)");
+  e = hipMalloc(reinterpret_cast<void**>(&v->d_decisions), max_sequences * sizeof(ets::Decision));
+  if (e != hipSuccess) return bail(e, "ets_verifier_create: hipMalloc(decisions)");
+  e = hipMalloc(reinterpret_cast<void**>(&v->d_token_logits), rows * sizeof(float));
+  if (e != hipSuccess) return bail(e, "ets_verifier_create: hipMalloc(token logits)");
   e = hipMalloc(reinterpret_cast<void**>(&v->d_exp2), ets::kExp2Steps * sizeof(double));
   if (e != hipSuccess) return bail(e, "ets_verifier_create: hipMalloc(table)");
   double table[ets::kExp2Steps];
@@ -111,7 +113,9 @@ ets_status ets_verifier_destroy(ets_verifier* v) {
   {
     ets_host::DeviceGuard g(v->device);
     (void)hipFree(v->d_stats);
-    (void)hipFree(v->d_rest);
+    (void)hipFree(v->d_mass);
+    (void)hipFree(v->d_decisions);
+    (void)hipFree(v->d_token_logits);
     (void)hipFree(v->d_exp2);
   }
   delete v;
@@ -165,19 +169,22 @@ ets_status ets_verifier_verify(ets_verifier* v, const ets_verify_batch* a, void*
   p.tokens_stride = a->tokens_stride;
   p.accepted = a->accepted;
   p.vocab = v->vocab;
+  p.chunks = chunks_of(v->vocab);
   p.drafts = a->drafts;
   p.sequences = a->sequences;
   p.rows_per_seq = p.draft ? 2 * a->drafts + 1 : a->drafts + 1;
   p.stats = v->d_stats;
-  p.rest = v->d_rest;
+  p.token_logits = v->d_token_logits;
+  p.decisions = v->d_decisions;
+  p.mass = v->d_mass;
   p.exp2_table = v->d_exp2;
   ets_host::DeviceGuard g(v->device);
   hipStream_t stream = static_cast<hipStream_t>(hip_stream);
   hipError_t e = hipSuccess;
   switch (a->dtype) {
-    case ETS_DTYPE_FLOAT: e = launch_verify<ets::kDtypeFloat>(p, stream); break;
-    case ETS_DTYPE_HALF: e = launch_verify<ets::kDtypeHalf>(p, stream); break;
-    default: e = launch_verify<ets::kDtypeBFloat16>(p, stream); break;
+    case ETS_DTYPE_FLOAT: e = launch_verify<ets::kDtypeFloat>(p, v->num_cus, stream); break;
+    case ETS_DTYPE_HALF: e = launch_verify<ets::kDtypeHalf>(p, v->num_cus, stream); break;
+    default: e = launch_verify<ets::kDtypeBFloat16>(p, v->num_cus, stream); break;
   }
   return e == hipSuccess ? ETS_OK : verifier_hip_fail(v, e, "ets_verifier_verify: launch");
 }

@@ -1,36 +1,73 @@
 // Kernels of the verification of drafted tokens (include/et_speculative.h).
 //
-// A sequence has K + 1 target rows and, with a draft model, K draft rows.  Three launches:
-//   verify_stats   every row is cut into chunks; a workgroup reduces one chunk to (max, sum of
-//                  exp((l - max) / T)), or, for a greedy sequence, to its best (key, ~index)
-//   verify_rest    (draft model only) per sequence: which position decides, then the mass of
-//                  max(p - q, 0) of every chunk of that position's rows
-//   verify_finish  one workgroup per sequence: the decision again, the chunk in which the drawn token
-//                  lies, and a scan of that chunk
-// The kernel boundaries order the three; nothing is handed over inside a launch, so a launch needs no
-// waits and leaves no state behind.
+// A sequence has K + 1 target rows and, with a draft model, K draft rows; each is cut into chunks.  Launches:
+//   verify_stats   (max, sum of exp((l - max) / T)) of every chunk of every row, in fp32; of a greedy
+//                  sequence's rows the best (key, ~index)
+//   verify_decide  per sequence: which drafts are kept, from coins and probabilities
+//   verify_rest    per sequence and chunk: the mass that the next token is drawn from, in 64 bits, of the one
+//                  position that decides (small batches decide in here, each workgroup for itself)
+//   verify_finish  per sequence: the chunk in which the drawn token lies, and a scan of it
+// The kernel boundaries order them; nothing is handed over inside a launch, so a launch needs no waits and
+// leaves no state behind.
 //
-// Weights are computed in 64 bits: a token is the place where a running sum over up to 2^18 weights
-// crosses a threshold, and an error e of that sum moves about e x (entries that matter) draws over a
-// border; at 1e-13 that is one draw in 1e8.  The 64-bit rate of the vector unit is its 32-bit rate, so
-// what this costs is registers and about twice the instructions of a 32-bit exponential.
+// Precision.  A draw is the place where a running sum over up to 2^18 weights crosses a threshold, and an
+// error e of that sum moves about e x (entries that matter) draws over a border: at fp32's 1e-7 that is a
+// wrong token in a few hundred flat rows, so masses are held in 64 bits.  That costs some
+// 20 instructions an entry and is spent on one row pair a sequence.  The statistics of all rows take 6
+// instructions an entry, which keeps them at the speed of memory; they only decide about acceptance, and
+// where coin * q and p are closer than their error allows, verify_decide sums the two rows again in 64 bits.
 #pragma once
 
 #include "ets_kernels.h"
 
 namespace ets {
 
-constexpr int kVerifyBlock = 256;    // lanes of verify_stats and verify_rest
-constexpr int kFinishBlock = 1024;   // lanes of verify_finish
+constexpr int kVerifyBlock = 256;    // lanes of a workgroup
+constexpr int kVerifyWaves = kVerifyBlock / 64;
 constexpr int kMaxDrafts = 64;       // drafts per sequence: one lane of a wave each
-constexpr int kExp2Steps = 256;      // entries of the table of 2^(j / 256)
-constexpr int kSmallChunk = 2048, kLargeChunk = 8192;  // entries per chunk
+constexpr int kVerifyChunk = 2048;   // entries per chunk of a row
+constexpr int kLaneEntries = kVerifyChunk / kVerifyBlock;
+constexpr int kExp2Steps = 32;       // entries of the table of 2^(j / 32)
+constexpr double kLog2E = 1.44269504088896340736;
+constexpr double kEmptyRest = 1.0 / (1 << 30);  // residual masses up to this are rounding noise of p - q
 
 struct ChunkStat {
   double sum;   // of exp((l - max) / T); NaN where the chunk holds a NaN or +inf (greedy: the bits of the best key)
   float max;
   float pad;
 };
+
+struct RowNorm {
+  double sum;  // of exp((l - max) / T) over the row; not above 0 where the row has no distribution
+  float max;
+  int32_t best;  // greedy sequences: the row's arg-max
+};
+
+struct Decision {
+  double rho;      // (sum of the target row) / (sum of the draft row) at `kept`, as the statistics have it
+  int kept;        // drafts accepted
+  int draw;        // kDraw*: what the next token is drawn from
+  int skip;        // kDrawWithout: the token left out
+  float temperature;
+  float t_max, d_max;  // of the rows at `kept`
+  int answer;      // kDrawNone: the next token
+  int pad;
+};
+constexpr int kDrawNone = 0;     // nothing is drawn: a greedy sequence, or a row without a distribution
+constexpr int kDrawTarget = 1;   // p
+constexpr int kDrawWithout = 2;  // p without one token
+constexpr int kDrawRest = 3;     // max(p - q, 0)
+
+// Of a chunk of the deciding rows, with a = exp((t - t_max) / T), b = exp((d - d_max) / T), skipped or not:
+struct ChunkMass {
+  double all;   // sum of a
+  double draft; // sum of b
+  double rest;  // kDrawRest: sum of max(a - rho b, 0); otherwise of a without the token left out
+  double over;  // kDrawRest: sum of b where a - rho b > 0
+  double edge;  // kDrawRest: sum of b where |a - rho b| < kEdge a
+  double pad;
+};
+constexpr double kEdge = 1.0 / (1 << 20);
 
 struct VerifyParams {
   const void* target;
@@ -49,8 +86,11 @@ struct VerifyParams {
   int32_t vocab, drafts, sequences;
   int32_t chunks;          // per row
   int32_t rows_per_seq;    // K + 1, or 2K + 1 with a draft model
+  int32_t step_b, step_j, step_chunk;  // how far apart a wave's chunks are in verify_stats
   ChunkStat* stats;        // [sequences, rows_per_seq, chunks]
-  double* rest;            // [sequences, chunks]
+  float* token_logits;     // [sequences, rows_per_seq]: of the row's drafted token
+  Decision* decisions;     // [sequences]
+  ChunkMass* mass;         // [sequences, chunks]
   const double* exp2_table;
 };
 
@@ -60,17 +100,26 @@ struct __attribute__((packed, aligned(DT == kDtypeFloat ? 4 : 2))) LooseVec {
   uint32_t w[4];
 };
 
+template <int DT>
+__device__ __forceinline__ uint4 load_whole(const char* row, int first) {
+  const LooseVec<DT> v = *reinterpret_cast<const LooseVec<DT>*>(row + static_cast<int64_t>(first) * ElemSize<DT>::value);
+  return make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+}
+
+template <int DT>
+__device__ __forceinline__ uint4 load_none() {  // -inf throughout
+  constexpr uint32_t kFill = DT == kDtypeFloat ? 0xff800000u : (DT == kDtypeBFloat16 ? 0xff80ff80u : 0xfc00fc00u);
+  return make_uint4(kFill, kFill, kFill, kFill);
+}
+
 // Entries [first, first + VecElems) of a row as raw bits; those at n and behind read as -inf and are
 // not touched in memory.
 template <int DT>
 __device__ __forceinline__ uint4 load_raw(const char* row, int first, int n) {
-  constexpr int VE = VecElems<DT>::value, ES = ElemSize<DT>::value;
-  if (first + VE <= n) {
-    const LooseVec<DT> v = *reinterpret_cast<const LooseVec<DT>*>(row + static_cast<int64_t>(first) * ES);
-    return make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
-  }
-  constexpr uint32_t kFill = DT == kDtypeFloat ? 0xff800000u : (DT == kDtypeBFloat16 ? 0xff80ff80u : 0xfc00fc00u);
-  uint32_t w[4] = {kFill, kFill, kFill, kFill};
+  constexpr int VE = VecElems<DT>::value;
+  if (first + VE <= n) return load_whole<DT>(row, first);
+  const uint4 none = load_none<DT>();
+  uint32_t w[4] = {none.x, none.y, none.z, none.w};
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
     if (first + e < n) {
@@ -85,32 +134,44 @@ __device__ __forceinline__ uint4 load_raw(const char* row, int first, int n) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// exp((l - m) / T) for l <= m, c = 256 log2(e) / T: 2^(k/256) 2^(r/256) with k = round((l - m) c), the
-// first factor from the table (a copy in LDS) and k's high bits, the second, |r| <= 1/2, by its series to
-// the third power: the first term left out is (ln 2 / 512)^4 / 24 = 1.4e-13.  l = -inf gives 0, whatever T:
-// the argument is cut off where the result is 0 (fmax also drops the NaN of -inf * 0 at T = inf).
-__device__ __forceinline__ double exp_weight(float l, double m, double c, const double* table) {
-  constexpr double kStep = 0.69314718055994530942 / kExp2Steps;
-  const double t = fmax((static_cast<double>(l) - m) * c, -600000.0);
-  const double kd = __builtin_rint(t);
-  const double r = t - kd;
-  const int k = static_cast<int>(kd);
-  const double poly = fma(r, fma(r, fma(r, kStep * kStep * kStep / 6.0, kStep * kStep / 2.0), kStep), 1.0);
-  return ldexp(poly * table[k & (kExp2Steps - 1)], k >> 8);
-}
-
-// The same for one entry, without the table.
+// ---- weights ------------------------------------------------------------------------------------
+// exp((l - m) / T), in 64 bits, of one entry.
 __device__ __forceinline__ double exact_weight(float l, float m, float temperature) {
   return l == -INFINITY ? 0.0 : exp((static_cast<double>(l) - m) / temperature);
 }
 
-__device__ __forceinline__ double temperature_factor(float temperature) {
-  return (kExp2Steps * 1.44269504088896340736) / static_cast<double>(temperature);
-}
+// The same of many entries of a row: 2^(k/32) 2^(r/32) with k = round((l - m) c), c = 32 log2(e) / T.  Adding
+// 1.5 * 2^52 leaves k in the low word of the sum; the first factor comes from a table of 32 doubles (one LDS
+// bank pair each, so lanes never wait for each other) and k's upper bits, the second, |r| <= 1/2, from its
+// series to the fifth power with the sixth term spread over the fourth and the second (its Chebyshev
+// expansion), which leaves 2e-16: a residual p - q of nearly equal models is a difference of weights, and the
+// rounding of the weights is what is left of it.  l - m is cut off at -800 T, where the result is 0.  A weight
+// of 1 (l = m) is exact.
+struct RowWeights {
+  static constexpr double kStep = 0.69314718055994530942 / kExp2Steps;
+  double m, lowest, c, c5, c4, c3, c2, c1;
+  __device__ __forceinline__ RowWeights(float max, float temperature) {
+    m = max;
+    lowest = -800.0 * temperature;
+    c = kExp2Steps * kLog2E / static_cast<double>(temperature);
+    constexpr double h = kStep, h6 = h * h * h * h * h * h / 720.0;
+    c5 = h * h * h * h * h / 120.0, c4 = h * h * h * h / 24.0 + 0.375 * h6, c3 = h * h * h / 6.0, c2 = h * h / 2.0 - 0.03515625 * h6, c1 = h;
+    asm("" : "+v"(c5), "+v"(c4), "+v"(c3), "+v"(c2), "+v"(c1));  // (kept in registers: as literals they would be moved there for every entry)
+  }
+  __device__ __forceinline__ double operator()(float l, const double* table) const {
+    constexpr double kShift = 0x1.8p52;
+    const double d = fmax(static_cast<double>(l) - m, lowest);
+    const double sum = fma(d, c, kShift);
+    const int k = __double2loint(sum);
+    const double r = fma(d, c, kShift - sum);  // (kShift - sum is -k: exact)
+    const double power = fma(r, fma(r, fma(r, fma(r, fma(r, c5, c4), c3), c2), c1), 1.0) * table[k & (kExp2Steps - 1)];
+    return ldexp(power, k >> 5);
+  }
+};
 
 __device__ __forceinline__ float sequence_temperature(const VerifyParams& p, int b) {
   const float t = p.temperatures ? p.temperatures[b] : p.temperature;
-  return t < 0.0f ? 0.0f : t;
+  return t > 0.0f ? fminf(fmaxf(t, 1e-30f), 1e30f) : (t <= 0.0f ? 0.0f : t);  // (NaN stays)
 }
 
 __device__ __forceinline__ int sequence_length(const VerifyParams& p, int b) {
@@ -126,16 +187,25 @@ __device__ __forceinline__ const char* draft_row(const VerifyParams& p, int b, i
   return static_cast<const char*>(p.draft) + (b * p.draft_seq + i * p.draft_pos) * ElemSize<DT>::value;
 }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+// Inclusive prefix sum over the 64 lanes by DPP steps (row shifts, then row broadcasts), in a fixed order.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ double dpp_or_zero_f64(double v) {
+  return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROW_MASK, 0xf, false),
+                          __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROW_MASK, 0xf, false));
+}
+__device__ __forceinline__ double wave_scan_f64(double v) {
+  v += dpp_or_zero_f64<0x111, 0xf>(v);
+  v += dpp_or_zero_f64<0x112, 0xf>(v);
+  v += dpp_or_zero_f64<0x114, 0xf>(v);
+  v += dpp_or_zero_f64<0x118, 0xf>(v);
+  v += dpp_or_zero_f64<0x142, 0xa>(v);
+  v += dpp_or_zero_f64<0x143, 0xc>(v);
   return v;
 }
-__device__ __forceinline__ float wave_max_f32(float v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-  return v;
+__device__ __forceinline__ double lane_f64(double v, int lane) {  // (`lane`: the same in every lane)
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
 }
+__device__ __forceinline__ double wave_sum_f64(double v) { return lane_f64(wave_scan_f64(v), 63); }
 
 // Sum over the workgroup, in a fixed order; every lane gets it.  `red`: one double per wave.
 template <int WAVES>
@@ -151,392 +221,550 @@ __device__ __forceinline__ double block_sum_f64(double v, double* red) {
 }
 
 // ---- statistics of every chunk ------------------------------------------------------------------
-// U vectors per lane, all of them in registers: the chunk is read once, its maximum found, then its sum.
-template <int DT, int U>
-__global__ void __launch_bounds__(kVerifyBlock)
-verify_stats_kernel(const VerifyParams p) {
-  constexpr int VE = VecElems<DT>::value;
-  constexpr int kWavesHere = kVerifyBlock / 64;
-  __shared__ double table[kExp2Steps];
-  __shared__ float red_max[kWavesHere];
-  __shared__ int red_bad[kWavesHere];
-  __shared__ double red_sum[kWavesHere];
-  __shared__ uint64_t red_best[kWavesHere];
-  const int tid = threadIdx.x, wave = tid >> 6;
-  const int row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
-  const int b = row / p.rows_per_seq, j = row - b * p.rows_per_seq;
-  const bool is_draft = j > p.drafts;
-  const int pos = is_draft ? j - p.drafts - 1 : j;
-  const int len = sequence_length(p, b);
-  if (is_draft ? pos >= len : pos > len) return;  // (the row is not the sequence's)
-  const float temperature = sequence_temperature(p, b);
-  const bool greedy = temperature == 0.0f;
-  if (is_draft && greedy) return;
-  const char* src = is_draft ? draft_row<DT>(p, b, pos) : target_row<DT>(p, b, pos);
-  const int first = chunk * (kVerifyBlock * VE * U);
-  ChunkStat* out = p.stats + static_cast<int64_t>(row) * p.chunks + chunk;
+// A wave takes one chunk after the other, `stride` of them apart; a chunk is read once, into registers, its
+// maximum found and then its sum, while the next chunk is on its way.  Waves need nothing from each
+// other, so there are no barriers.
+struct ChunkCursor {  // (the same in every lane)
+  int b, j, chunk;    // sequence, row of the sequence, chunk of the row
+  bool there;         // within the batch
+  __device__ __forceinline__ void start(const VerifyParams& p, int item) {
+    const int row = item / p.chunks;
+    chunk = item - row * p.chunks;
+    b = row / p.rows_per_seq;
+    j = row - b * p.rows_per_seq;
+    there = b < p.sequences;
+  }
+  __device__ __forceinline__ void step(const VerifyParams& p) {
+    chunk += p.step_chunk;
+    j += p.step_j;
+    b += p.step_b;
+    if (chunk >= p.chunks) chunk -= p.chunks, j += 1;
+    if (j >= p.rows_per_seq) j -= p.rows_per_seq, b += 1;
+    there = b < p.sequences;
+  }
+};
 
+template <int DT>
+struct ChunkData {
+  static constexpr int VE = VecElems<DT>::value, U = kVerifyChunk / 64 / VE;
   uint4 raw[U];
+  const char* src;
+  float temperature;
+  int pos, len;
+  bool wanted;  // the row is one of the sequence's, and is looked at
+  __device__ __forceinline__ void load(const VerifyParams& p, const ChunkCursor& at) {
+    wanted = false;
+    if (!at.there) return;
+    const bool is_draft = at.j > p.drafts;
+    pos = is_draft ? at.j - p.drafts - 1 : at.j;
+    len = sequence_length(p, at.b);
+    temperature = sequence_temperature(p, at.b);
+    if (is_draft ? pos >= len || temperature == 0.0f : pos > len) return;
+    wanted = true;
+    src = is_draft ? draft_row<DT>(p, at.b, pos) : target_row<DT>(p, at.b, pos);
+    const int lane = threadIdx.x & 63, first = at.chunk * kVerifyChunk, n = p.vocab - first;
+    if (n >= kVerifyChunk) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) raw[u] = load_raw<DT>(src, first + (u * kVerifyBlock + tid) * VE, p.vocab);
-  for (int i = tid; i < kExp2Steps; i += kVerifyBlock) table[i] = p.exp2_table[i];
-
-  if (greedy) {
-    uint64_t best = 0;
+      for (int u = 0; u < U; ++u) raw[u] = load_whole<DT>(src, first + (u * 64 + lane) * VE);
+    } else {  // the row's last chunk: whole vectors, one that is cut short (at most), and nothing
+      const int cut = n / VE;
+      const uint4 short_one = load_raw<DT>(src, first + (lane == (cut & 63) ? cut * VE : n), p.vocab);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float v[VE];
-      decode_vec<DT>(raw[u], v);
-      const int at = first + (u * kVerifyBlock + tid) * VE;
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const uint64_t key = pack_best(order_key(v[e]), at + e);
-        if (at + e < p.vocab && key > best) best = key;
+      for (int u = 0; u < U; ++u) {
+        const int vec = u * 64 + lane;
+        raw[u] = vec < cut ? load_whole<DT>(src, first + vec * VE) : short_one;
+        if (vec > cut) raw[u] = load_none<DT>();
       }
     }
-    best = wave_max_u64(best);
-    if ((tid & 63) == 0) red_best[wave] = best;
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < kWavesHere; ++w) best = red_best[w] > best ? red_best[w] : best;
-      out->sum = __longlong_as_double(static_cast<long long>(best));
-    }
-    return;
   }
+};
 
+// The sum's error, relative: an entry's exponent t is rounded three times (l - m, the factor c, their product),
+// by at most |t| 2^-24 each, the exponential by 2^-23, the additions of a lane by 2^-24 each, eight of them;
+// the weighted mean of |t| over a row is below log2 of its length, at most 24.  (3 * 24 ln 2 + 2 + 8) 2^-24 < 60 * 2^-24.
+constexpr double kStatError = 60.0 / (1 << 24);
+
+template <int DT>
+__device__ __forceinline__ void chunk_stat(const VerifyParams& p, const ChunkCursor& at, const ChunkData<DT>& d) {
+  constexpr int VE = ChunkData<DT>::VE, U = ChunkData<DT>::U;
+  const int lane = threadIdx.x & 63;
+  const int row = at.b * p.rows_per_seq + at.j;
+  const int first = at.chunk * kVerifyChunk, end = min(first + kVerifyChunk, p.vocab);
+  ChunkStat* out = p.stats + static_cast<int64_t>(row) * p.chunks + at.chunk;
   float m = -INFINITY;
-  int bad = 0;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float v[VE];
-    decode_vec<DT>(raw[u], v);
+    decode_vec<DT>(d.raw[u], v);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      m = fmaxf(m, v[e]);
-      bad |= v[e] != v[e];
-    }
+    for (int e = 0; e < VE; ++e) m = fmaxf(m, v[e]);  // (drops NaN)
   }
-  m = wave_max_f32(m);
-  bad = __any(bad);
-  if ((tid & 63) == 0) red_max[wave] = m, red_bad[wave] = bad;
-  __syncthreads();
+  m = wave_max_ignoring_nan(m);
+  if (d.temperature == 0.0f) {
+    int best = end;
 #pragma unroll
-  for (int w = 0; w < kWavesHere; ++w) m = fmaxf(m, red_max[w]), bad |= red_bad[w];
-  if (bad || m == INFINITY || m == -INFINITY || temperature != temperature) {  // (the same in every lane)
-    if (tid == 0) {
-      out->max = m;
-      out->sum = (m == -INFINITY && !bad && temperature == temperature) ? 0.0 : static_cast<double>(NAN);
+    for (int u = U - 1; u >= 0; --u) {
+      float v[VE];
+      decode_vec<DT>(d.raw[u], v);
+#pragma unroll
+      for (int e = VE - 1; e >= 0; --e) best = v[e] == m ? first + (u * 64 + lane) * VE + e : best;
+    }
+    best = -wave_max_i32(-best);
+    // (nothing equals the maximum: NaN throughout, the key 0)
+    if (lane == 0) {
+      const uint64_t key = best < end ? pack_best(order_key(m), best) : pack_best(0u, first);
+      out->sum = __longlong_as_double(static_cast<long long>(key));
     }
     return;
   }
-  const double c = temperature_factor(temperature), md = m;
-  double sum = 0.0;
+  if (lane == 0 && d.pos < d.len) {
+    const int x = p.draft_tokens[at.b * p.draft_tokens_stride + d.pos];
+    if (x >= first && x < end) p.token_logits[row] = load_elem<DT>(d.src, x);
+  }
+  // 2^((l - m) c): -inf gives 0, NaN and a maximum of +inf come out in the sum as NaN
+  const float c = static_cast<float>(kLog2E) / d.temperature, from = m == -INFINITY ? 0.0f : m;
+  float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float v[VE];
-    decode_vec<DT>(raw[u], v);
+    decode_vec<DT>(d.raw[u], v);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) sum += exp_weight(v[e], md, c, table);
+    for (int e = 0; e < VE; ++e) part[e & 3] += __builtin_amdgcn_exp2f((v[e] - from) * c);
   }
-  sum = block_sum_f64<kWavesHere>(sum, red_sum);
-  if (tid == 0) {
+  const double sum = wave_sum_f64((static_cast<double>(part[0]) + part[1]) + (static_cast<double>(part[2]) + part[3]));
+  if (lane == 0) {
     out->max = m;
     out->sum = sum;
   }
 }
 
-// ---- the decision -------------------------------------------------------------------------------
-struct RowNorm {
-  double sum;  // of exp((l - max) / T) over the row; not above 0 where the row has no distribution
-  float max;
-  int32_t best;  // greedy sequences: the row's arg-max
-};
-
-// One wave: the row's statistics from its chunks', in a fixed order.
-__device__ __forceinline__ RowNorm combine_chunks(const ChunkStat* st, int chunks, bool greedy, float temperature) {
-  const int lane = threadIdx.x & 63;
-  RowNorm r = {0.0, -INFINITY, 0};
-  if (greedy) {
-    uint64_t best = 0;
-    for (int c = lane; c < chunks; c += 64) {
-      const uint64_t k = static_cast<uint64_t>(__double_as_longlong(st[c].sum));
-      best = k > best ? k : best;
-    }
-    best = wave_max_u64(best);
-    r.best = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(best));
-    return r;
+template <int DT>
+__global__ void __launch_bounds__(kVerifyBlock)
+verify_stats_kernel(const VerifyParams p) {
+  ChunkCursor at;
+  at.start(p, __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * kVerifyWaves + (threadIdx.x >> 6))));
+  ChunkData<DT> d;
+  d.load(p, at);
+  while (at.there) {
+    ChunkCursor next = at;
+    next.step(p);
+    ChunkData<DT> ahead;
+    ahead.load(p, next);
+    if (d.wanted) chunk_stat<DT>(p, at, d);
+    at = next;
+    d = ahead;
   }
-  float m = -INFINITY;
-  for (int c = lane; c < chunks; c += 64) m = fmaxf(m, st[c].max);
-  m = wave_max_f32(m);
-  double s = 0.0;
-  for (int c = lane; c < chunks; c += 64) {
-    const double sc = st[c].sum;  // (a chunk without a finite entry: 0; exp(-inf) stays out of the sum)
-    s += st[c].max == -INFINITY ? sc : sc * exact_weight(st[c].max, m, temperature);
-  }
-  r.max = m;
-  r.sum = wave_sum_f64(s);
-  return r;
 }
 
-struct Decision {
-  int kept;        // drafts accepted
-  int len;         // the sequence's drafts
-  int valid;       // 0: a row at `kept` has no distribution
-  int best;        // greedy: the arg-max of the target row at `kept`
-  float temperature;
-  RowNorm t, d;    // rows at `kept` (d: with draft logits and kept < len only)
+// ---- the decision -------------------------------------------------------------------------------
+// One wave: the statistics of R rows from their chunks', in a fixed order; the first 64 chunks of all R
+// rows are on their way together.
+template <int R>
+__device__ __forceinline__ void combine_chunks(const ChunkStat* const* st, int chunks, bool greedy, float temperature, RowNorm* out) {
+  const int lane = threadIdx.x & 63;
+  double s[R];
+  float m[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    s[r] = 0.0, m[r] = -INFINITY;
+    if (lane < chunks) s[r] = st[r][lane].sum, m[r] = st[r][lane].max;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    RowNorm n = {0.0, -INFINITY, 0};
+    if (greedy) {
+      uint64_t best = static_cast<uint64_t>(__double_as_longlong(s[r]));  // (+0.0, the key 0, where there is no chunk)
+      for (int c = lane + 64; c < chunks; c += 64) {
+        const uint64_t k = static_cast<uint64_t>(__double_as_longlong(st[r][c].sum));
+        best = k > best ? k : best;
+      }
+      n.best = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(wave_max_u64(best)));
+    } else {
+      float top = m[r];
+      for (int c = lane + 64; c < chunks; c += 64) top = fmaxf(top, st[r][c].max);
+      top = wave_max_ignoring_nan(top);
+      // (a chunk without a finite entry has the sum 0, or NaN, and no exponential)
+      double sum = m[r] == -INFINITY ? s[r] : s[r] * exact_weight(m[r], top, temperature);
+      for (int c = lane + 64; c < chunks; c += 64) {
+        const ChunkStat k = st[r][c];
+        sum += k.max == -INFINITY ? k.sum : k.sum * exact_weight(k.max, top, temperature);
+      }
+      n.max = top;
+      n.sum = wave_sum_f64(sum);
+    }
+    out[r] = n;
+  }
+}
+
+struct DecideSpace {  // in LDS
+  RowNorm rows[2 * kMaxDrafts + 1];
+  double table[kExp2Steps];
+  double red[kVerifyWaves];
+  uint64_t near;  // drafts whose coin is too close to tell
+  uint64_t accept, valid;
 };
 
-// Which position decides, worked out by the whole workgroup of WAVES waves from the statistics (every
-// workgroup that needs it does so for itself: it is a few hundred bytes and one exponential per draft).
-template <int DT, int WAVES>
-__device__ __forceinline__ Decision decide(const VerifyParams& p, int b, RowNorm* rows /* [2 kMaxDrafts + 1], LDS */, int* shared /* LDS */) {
+// The row's sum in 64 bits, by the whole workgroup.
+template <int DT>
+__device__ __forceinline__ double exact_sum(const VerifyParams& p, const char* row, float max, float temperature, DecideSpace& lds) {
+  const RowWeights weight(max, temperature);
+  double sum = 0.0;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < p.vocab; i += kVerifyBlock) sum += weight(load_elem<DT>(row, i), lds.table);
+  return block_sum_f64<kVerifyWaves>(sum, lds.red);
+}
+
+// What happens to a sequence, worked out by a workgroup from the statistics (in small batches every
+// workgroup of verify_rest does so for itself: it is a few hundred bytes and two exponentials per draft).
+template <int DT>
+__device__ __forceinline__ Decision decide(const VerifyParams& p, int b, DecideSpace& lds) {
+  constexpr int R = 3;
   const int tid = threadIdx.x, wave = tid >> 6;
   Decision out;
-  out.len = sequence_length(p, b);
-  out.temperature = sequence_temperature(p, b);
-  const bool greedy = out.temperature == 0.0f;
-  const ChunkStat* st = p.stats + static_cast<int64_t>(b) * p.rows_per_seq * p.chunks;
-  for (int j = wave; j < p.rows_per_seq; j += WAVES) {
-    const bool is_draft = j > p.drafts;
-    const int pos = is_draft ? j - p.drafts - 1 : j;
-    if ((is_draft && greedy) || (is_draft ? pos >= out.len : pos > out.len)) continue;
-    const RowNorm r = combine_chunks(st + static_cast<int64_t>(j) * p.chunks, p.chunks, greedy, out.temperature);
-    if ((tid & 63) == 0) rows[j] = r;
+  const int len = sequence_length(p, b);
+  const float temperature = sequence_temperature(p, b);
+  out.temperature = temperature;
+  const bool greedy = temperature == 0.0f;
+  const int64_t row0 = static_cast<int64_t>(b) * p.rows_per_seq;
+  const ChunkStat* st = p.stats + row0 * p.chunks;
+  if (tid < kExp2Steps) lds.table[tid] = p.exp2_table[tid];
+  // of this lane's draft, whatever the statistics say
+  int x = -1;
+  float coin = 0.0f, t_logit = 0.0f, d_logit = 0.0f;
+  if (tid < len && tid < 64) {
+    x = p.draft_tokens[b * p.draft_tokens_stride + tid];
+    if (!greedy && x >= 0 && x < p.vocab) {
+      coin = p.coins[b * p.coins_stride + tid];
+      t_logit = p.token_logits[row0 + tid];
+      if (p.draft) d_logit = p.token_logits[row0 + p.drafts + 1 + tid];
+    }
+  }
+  const bool inside = x >= 0 && x < p.vocab;
+  // the sequence's rows: target 0 .. len, and draft 0 .. len - 1 unless it is greedy
+  const int count = len + 1 + (p.draft && !greedy ? len : 0);
+  for (int k = wave * R; k < count; k += kVerifyWaves * R) {
+    const ChunkStat* src[R];
+    RowNorm norm[R];
+    int at[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int j = min(k + r, count - 1);  // (a row too many is worked out again)
+      at[r] = j <= len ? j : p.drafts + j - len;
+      src[r] = st + static_cast<int64_t>(at[r]) * p.chunks;
+    }
+    combine_chunks<R>(src, p.chunks, greedy, temperature, norm);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if ((tid & 63) == 0) lds.rows[at[r]] = norm[r];
+    }
   }
   __syncthreads();
   if (wave == 0) {
-    bool accept = false, valid = true;
-    if (tid <= out.len) {
-      const RowNorm t = rows[tid];
+    bool accept = false, valid = true, near = false;
+    if (tid <= len) {
+      const RowNorm t = lds.rows[tid];
       valid = greedy || t.sum > 0.0;
-      if (tid < out.len) {
-        const int x = p.draft_tokens[b * p.draft_tokens_stride + tid];
+      if (tid < len) {
         if (greedy) {
           accept = x == t.best;
         } else {
           double q = 1.0;
           if (p.draft) {
-            const RowNorm d = rows[p.drafts + 1 + tid];
+            const RowNorm d = lds.rows[p.drafts + 1 + tid];
             valid = valid && d.sum > 0.0;
-            if (x >= 0 && x < p.vocab)
-              q = exact_weight(load_elem<DT>(draft_row<DT>(p, b, tid), x), d.max, out.temperature) / d.sum;
+            if (inside) q = exact_weight(d_logit, d.max, temperature) / d.sum;
           }
-          if (valid && x >= 0 && x < p.vocab) {
-            const double pt = exact_weight(load_elem<DT>(target_row<DT>(p, b, tid), x), t.max, out.temperature) / t.sum;
-            accept = static_cast<double>(p.coins[b * p.coins_stride + tid]) * q < pt;
+          if (valid && inside) {
+            const double pt = exact_weight(t_logit, t.max, temperature) / t.sum, cq = static_cast<double>(coin) * q;
+            accept = cq < pt;
+            near = fabs(cq - pt) <= 2.0 * kStatError * (1.0 + 1e-3) * pt && pt > 0.0;  // (both sums' errors)
           }
         }
       }
     }
-    // (lane 64 does not exist: with 64 drafts the row behind the last one is looked at below)
-    const uint64_t stop = __ballot(tid < out.len && !accept);
-    const int kept = stop ? __ffsll(static_cast<unsigned long long>(stop)) - 1 : out.len;
-    const uint64_t good = __ballot(valid);
-    if (tid == 0) {
-      shared[0] = kept;
-      shared[1] = kept < 64 ? static_cast<int>((good >> kept) & 1) : (greedy || rows[kept].sum > 0.0);
-    }
+    const uint64_t accepts = __ballot(accept), goods = __ballot(valid), nears = __ballot(near);
+    if (tid == 0) lds.accept = accepts, lds.valid = goods, lds.near = nears;
   }
   __syncthreads();
-  out.kept = shared[0];
-  out.valid = shared[1];
-  out.t = rows[out.kept];
-  out.best = out.t.best;
-  if (p.draft && out.kept < out.len && !greedy) {
-    out.d = rows[p.drafts + 1 + out.kept];
+  const uint64_t drafts = len < 64 ? (1ull << len) - 1 : ~0ull;
+  uint64_t accepts = lds.accept, nears = lds.near;
+  auto first_stop = [&] {
+    const uint64_t stop = ~accepts & drafts;
+    return stop ? __ffsll(static_cast<unsigned long long>(stop)) - 1 : len;
+  };
+  while (nears) {  // (rare: a few in 1e5 drafts)
+    const int i = __ffsll(static_cast<unsigned long long>(nears)) - 1;
+    if (i > first_stop()) break;
+    nears &= nears - 1;
+    const RowNorm t = lds.rows[i], d = p.draft ? lds.rows[p.drafts + 1 + i] : RowNorm{1.0, 0.0f, 0};
+    const double t_sum = exact_sum<DT>(p, target_row<DT>(p, b, i), t.max, temperature, lds);
+    const double d_sum = p.draft ? exact_sum<DT>(p, draft_row<DT>(p, b, i), d.max, temperature, lds) : 1.0;
+    if (tid == i) {
+      const double q = p.draft ? exact_weight(d_logit, d.max, temperature) / d_sum : 1.0;
+      const bool accept = static_cast<double>(coin) * q < exact_weight(t_logit, t.max, temperature) / t_sum;
+      lds.accept = accept ? accepts | (1ull << i) : accepts & ~(1ull << i);
+    }
+    __syncthreads();
+    accepts = lds.accept;
+  }
+  out.kept = first_stop();
+  const RowNorm t = lds.rows[out.kept];
+  // (the row behind the 64th draft has no lane of its own)
+  const bool valid = out.kept < 64 ? (lds.valid >> out.kept) & 1 : (greedy || t.sum > 0.0);
+  const bool rejected = out.kept < len;
+  out.t_max = t.max;
+  out.d_max = 0.0f;
+  out.rho = 0.0;
+  out.skip = -1;
+  out.answer = -1;
+  out.pad = 0;
+  if (!valid || greedy) {
+    out.draw = kDrawNone;
+    out.answer = valid ? t.best : -1;
+  } else if (!rejected) {
+    out.draw = kDrawTarget;
+  } else if (p.draft) {
+    const RowNorm d = lds.rows[p.drafts + 1 + out.kept];
+    out.draw = kDrawRest;
+    out.d_max = d.max;
+    out.rho = t.sum / d.sum;
   } else {
-    out.d = RowNorm{1.0, 0.0f, 0};
+    const int token = p.draft_tokens[b * p.draft_tokens_stride + out.kept];
+    out.draw = token >= 0 && token < p.vocab ? kDrawWithout : kDrawTarget;
+    out.skip = token;
   }
   return out;
 }
 
-// max(p - q, 0) of one entry.
-__device__ __forceinline__ double rest_weight(float t, float d, const Decision& dec, double c, double inv_t, double inv_d,
-                                              const double* table) {
-  return fmax(exp_weight(t, dec.t.max, c, table) * inv_t - exp_weight(d, dec.d.max, c, table) * inv_d, 0.0);
+template <int DT>
+__global__ void __launch_bounds__(kVerifyBlock)
+verify_decide_kernel(const VerifyParams p) {
+  __shared__ DecideSpace lds;
+  const Decision dec = decide<DT>(p, blockIdx.x, lds);
+  if (threadIdx.x == 0) p.decisions[blockIdx.x] = dec;
 }
 
-// ---- mass of max(p - q, 0) per chunk ------------------------------------------------------------
-template <int DT, int U>
+// ---- mass of every chunk ------------------------------------------------------------------------
+// The residual max(a / Zt - b / Zd, 0) = max(a - rho b, 0) / Zt needs the rows' exact sums before its own can be
+// taken.  One pass does for both: with the statistics' rho, usually off by some 1e-7, and B the sum of b over
+// the entries where a > rho b, the sum of max(a - rho' b, 0) for the exact rho' is the sum found plus
+// (rho - rho') B, but for entries whose sign changes between rho and rho'.  Those are among the entries summed up
+// in `edge`, and each is off by at most |rho - rho'| b; verify_finish takes the masses anew with rho' where that
+// could matter (two models that are all but equal).
+template <int DT, bool DECIDED>
 __global__ void __launch_bounds__(kVerifyBlock)
 verify_rest_kernel(const VerifyParams p) {
-  constexpr int VE = VecElems<DT>::value;
-  constexpr int kWavesHere = kVerifyBlock / 64;
-  __shared__ double table[kExp2Steps];
-  __shared__ RowNorm rows[2 * kMaxDrafts + 1];
-  __shared__ int shared[2];
-  __shared__ double red[kWavesHere];
+  constexpr int VE = VecElems<DT>::value, U = kLaneEntries / VE;
+  __shared__ DecideSpace lds;
   const int tid = threadIdx.x;
   const int b = blockIdx.x / p.chunks, chunk = blockIdx.x - b * p.chunks;
-  for (int i = tid; i < kExp2Steps; i += kVerifyBlock) table[i] = p.exp2_table[i];
-  const Decision dec = decide<DT, kWavesHere>(p, b, rows, shared);
-  if (dec.kept >= dec.len || !dec.valid || dec.temperature == 0.0f) return;  // (the same in every lane)
-  const char* t_row = target_row<DT>(p, b, dec.kept);
-  const char* d_row = draft_row<DT>(p, b, dec.kept);
-  const int first = chunk * (kVerifyBlock * VE * U);
-  const double c = temperature_factor(dec.temperature), inv_t = 1.0 / dec.t.sum, inv_d = 1.0 / dec.d.sum;
-  double sum = 0.0;
-#pragma unroll 1
-  for (int u = 0; u < U; ++u) {
-    const int at = first + (u * kVerifyBlock + tid) * VE;
-    float tv[VE], dv[VE];
-    decode_vec<DT>(load_raw<DT>(t_row, at, p.vocab), tv);
-    decode_vec<DT>(load_raw<DT>(d_row, at, p.vocab), dv);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) sum += rest_weight(tv[e], dv[e], dec, c, inv_t, inv_d, table);
+  Decision dec;
+  if (DECIDED) {
+    dec = p.decisions[b];
+    if (tid < kExp2Steps) lds.table[tid] = p.exp2_table[tid];
+  } else {
+    dec = decide<DT>(p, b, lds);
+    if (chunk == 0 && tid == 0) p.decisions[b] = dec;
   }
-  sum = block_sum_f64<kWavesHere>(sum, red);
-  if (tid == 0) p.rest[static_cast<int64_t>(b) * p.chunks + chunk] = sum;
+  if (dec.draw == kDrawNone) return;  // (the same in every lane)
+  const bool minus_q = dec.draw == kDrawRest;
+  const char* t_row = target_row<DT>(p, b, dec.kept);
+  uint4 t_raw[U], d_raw[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) t_raw[u] = load_raw<DT>(t_row, chunk * kVerifyChunk + (u * kVerifyBlock + tid) * VE, p.vocab);
+  if (minus_q) {
+    const char* d_row = draft_row<DT>(p, b, dec.kept);
+#pragma unroll
+    for (int u = 0; u < U; ++u) d_raw[u] = load_raw<DT>(d_row, chunk * kVerifyChunk + (u * kVerifyBlock + tid) * VE, p.vocab);
+  }
+  const RowWeights t_weight(dec.t_max, dec.temperature), d_weight(dec.d_max, dec.temperature);
+  __syncthreads();
+  double all = 0.0, draft = 0.0, rest = 0.0, over = 0.0, edge = 0.0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float tv[VE], dv[VE];
+    decode_vec<DT>(t_raw[u], tv);
+    if (minus_q) decode_vec<DT>(d_raw[u], dv);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const double a = t_weight(tv[e], lds.table);
+      all += a;
+      if (minus_q) {
+        const double q = d_weight(dv[e], lds.table), more = fma(-dec.rho, q, a);
+        draft += q;
+        rest += fmax(more, 0.0);
+        over += more > 0.0 ? q : 0.0;
+        const bool close = fabs(more) < kEdge * a;
+        if (__any(close)) edge += close ? q : 0.0;
+      } else {
+        rest += chunk * kVerifyChunk + (u * kVerifyBlock + tid) * VE + e == dec.skip ? 0.0 : a;
+      }
+    }
+  }
+  all = block_sum_f64<kVerifyWaves>(all, lds.red);
+  rest = block_sum_f64<kVerifyWaves>(rest, lds.red);
+  if (minus_q) {
+    draft = block_sum_f64<kVerifyWaves>(draft, lds.red);
+    over = block_sum_f64<kVerifyWaves>(over, lds.red);
+    edge = block_sum_f64<kVerifyWaves>(edge, lds.red);
+  }
+  if (tid == 0) p.mass[static_cast<int64_t>(b) * p.chunks + chunk] = ChunkMass{all, draft, rest, over, edge, 0.0};
 }
 
 // ---- the draw -----------------------------------------------------------------------------------
-constexpr double kEmptyRest = 1.0 / (1 << 30);  // residual masses up to this are rounding noise of p - q
-
-template <int DT, int CHUNK>
-__global__ void __launch_bounds__(kFinishBlock)
+template <int DT>
+__global__ void __launch_bounds__(kVerifyBlock)
 verify_finish_kernel(const VerifyParams p) {
-  constexpr int VE = VecElems<DT>::value;
-  constexpr int kWavesHere = kFinishBlock / 64;
-  constexpr int E = CHUNK / kFinishBlock < VE ? VE : CHUNK / kFinishBlock;  // consecutive entries per lane
-  static_assert(E % VE == 0 && CHUNK % E == 0 && CHUNK / E <= kFinishBlock, "lanes cover the chunk");
+  constexpr int VE = VecElems<DT>::value, E = kLaneEntries;  // consecutive entries per lane
   __shared__ double table[kExp2Steps];
-  __shared__ RowNorm rows[2 * kMaxDrafts + 1];
-  __shared__ int shared[2];
-  __shared__ double red[kWavesHere];
+  __shared__ double red[kVerifyWaves];
   __shared__ double pick_at;   // what is left of the threshold when the chunk begins
-  __shared__ int pick_chunk;
+  __shared__ double pick_rho;
+  __shared__ int pick_chunk, pick_draw, pick_again;
   __shared__ int found, last;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int b = blockIdx.x;
-  for (int i = tid; i < kExp2Steps; i += kFinishBlock) table[i] = p.exp2_table[i];
-  if (tid == 0) found = CHUNK, last = -1;
-  const Decision dec = decide<DT, kWavesHere>(p, b, rows, shared);
+  if (tid < kExp2Steps) table[tid] = p.exp2_table[tid];
+  if (tid == 0) found = kVerifyChunk, last = -1;
+  ChunkMass* mass = p.mass + static_cast<int64_t>(b) * p.chunks;
+  ChunkMass mass0 = {};  // of chunk `lane`: on its way while the decision is read
+  if (wave == 0 && lane < p.chunks) mass0 = mass[lane];
+  const int own = tid < p.drafts ? p.draft_tokens[b * p.draft_tokens_stride + tid] : -1;  // (before the answer is written: it may go to the same place)
+  const float coin = p.coins[b * p.coins_stride + p.drafts];
+  const Decision dec = p.decisions[b];
   int32_t* out = p.tokens + b * p.tokens_stride;
-  const int32_t* drafted = p.draft_tokens + b * p.draft_tokens_stride;
-  auto answer = [&](int token) {  // (by every lane, with the same token)
-    for (int i = tid; i <= p.drafts; i += kFinishBlock) out[i] = i < dec.kept ? drafted[i] : (i == dec.kept ? token : -1);
+  auto answer = [&](int token) {  // (by every lane, with the same token; kMaxDrafts is below the workgroup's size)
+    if (tid <= p.drafts) out[tid] = tid < dec.kept ? own : (tid == dec.kept ? token : -1);
     if (tid == 0) p.accepted[b] = dec.kept;
   };
-  if (!dec.valid) return answer(-1);
-  if (dec.temperature == 0.0f) return answer(dec.best);
+  if (dec.draw == kDrawNone) return answer(dec.answer);
 
-  const bool rejected = dec.kept < dec.len;
-  const char* t_row = target_row<DT>(p, b, dec.kept);
-  const char* d_row = p.draft && rejected ? draft_row<DT>(p, b, dec.kept) : t_row;
-  const double c = temperature_factor(dec.temperature), inv_t = 1.0 / dec.t.sum, inv_d = 1.0 / dec.d.sum;
-  const ChunkStat* st = p.stats + (static_cast<int64_t>(b) * p.rows_per_seq + dec.kept) * p.chunks;
-  const double* rest = p.rest + static_cast<int64_t>(b) * p.chunks;
-
-  // the weights of this lane's entries of a chunk: p (unnormalised), p without the entry `skip`, or p - q
-  auto weights = [&](int chunk, bool minus_q, int skip, double* w) {
-    const int at = chunk * CHUNK + tid * E;
-#pragma unroll
-    for (int g = 0; g < E / VE; ++g) {
-      float tv[VE], dv[VE];
-      const bool mine = tid * E < CHUNK;
-      decode_vec<DT>(load_raw<DT>(t_row, at + g * VE, mine ? p.vocab : 0), tv);
-      if (minus_q) decode_vec<DT>(load_raw<DT>(d_row, at + g * VE, mine ? p.vocab : 0), dv);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        w[g * VE + e] = minus_q ? rest_weight(tv[e], dv[e], dec, c, inv_t, inv_d, table)
-                                : (at + g * VE + e == skip ? 0.0 : exp_weight(tv[e], dec.t.max, c, table));
-      }
-    }
+  const RowWeights t_weight(dec.t_max, dec.temperature), d_weight(dec.d_max, dec.temperature);
+  auto chunk_mass = [&](int k) { return k < 64 ? mass0 : mass[k]; };
+  // of chunk k, if it is drawn from `draw`: the masses of kDrawRest carried from the statistics' rho to another
+  auto mass_of = [&](int k, int draw, double carry) {
+    if (k >= p.chunks) return 0.0;
+    const ChunkMass c = chunk_mass(k);
+    return draw == kDrawTarget ? c.all : (draw == kDrawWithout ? c.rest : fmax(fma(carry, c.over, c.rest), 0.0));
   };
-
-  // the mode: p - q of the draft model; p without the drafted token; p
-  bool minus_q = p.draft && rejected;
-  int skip = -1;
-  double skip_chunk_mass = 0.0;
-  if (!p.draft && rejected) {
-    const int x = drafted[dec.kept];
-    if (x >= 0 && x < p.vocab) {
-      // the mass of x's chunk without x, summed anew: p(x) may be all but 1, and a difference would cancel
-      skip = x;
-      double w[E], s = 0.0;
-      weights(x / CHUNK, false, skip, w);
-#pragma unroll
-      for (int e = 0; e < E; ++e) s += w[e];
-      skip_chunk_mass = block_sum_f64<kWavesHere>(s, red);
+  auto total_of = [&](int draw, double carry) {
+    double s = 0.0;
+    for (int k = lane; k < p.chunks; k += 64) s += mass_of(k, draw, carry);
+    return wave_sum_f64(s);
+  };
+  double all = 0.0, carry = 0.0, total = 0.0;  // (of the first wave)
+  if (wave == 0) {
+    double draft = 0.0, edge = 0.0;
+    for (int k = lane; k < p.chunks; k += 64) {
+      const ChunkMass c = chunk_mass(k);
+      all += c.all;
+      draft += c.draft;
+      edge += c.edge;
+    }
+    all = wave_sum_f64(all);
+    double rho = 0.0;
+    bool again = false;
+    if (dec.draw == kDrawRest) {
+      rho = all / wave_sum_f64(draft);
+      carry = dec.rho - rho;
+      edge = wave_sum_f64(edge);
+    }
+    total = total_of(dec.draw, carry);
+    // (`total` is not above the mass for rho: a convex function's tangent)
+    if (dec.draw == kDrawRest) again = fabs(carry) > 0.5 * kEdge * rho || fabs(carry) * edge > 1e-10 * total;
+    if (lane == 0) pick_rho = rho, pick_again = again;
+  }
+  __syncthreads();
+  const double rho = pick_rho;
+  if (pick_again) {  // (the same in every lane)
+    for (int k = 0; k < p.chunks; ++k) {
+      double sum = 0.0;
+      for (int i = k * kVerifyChunk + tid; i < min((k + 1) * kVerifyChunk, p.vocab); i += kVerifyBlock) {
+        const double a = t_weight(load_elem<DT>(target_row<DT>(p, b, dec.kept), i), table);
+        sum += fmax(fma(-rho, d_weight(load_elem<DT>(draft_row<DT>(p, b, dec.kept), i), table), a), 0.0);
+      }
+      sum = block_sum_f64<kVerifyWaves>(sum, red);
+      if (tid == 0) mass[k].rest = sum;
+    }
+    __syncthreads();
+    if (wave == 0) {
+      if (lane < p.chunks) mass0.rest = mass[lane].rest;
+      carry = 0.0;
+      total = total_of(kDrawRest, 0.0);
     }
   }
   if (wave == 0) {
-    auto mass = [&](int k) {
-      if (k >= p.chunks) return 0.0;
-      if (minus_q) return rest[k];
-      if (skip >= 0 && k == skip / CHUNK) return skip_chunk_mass;
-      return st[k].sum * exact_weight(st[k].max, dec.t.max, dec.temperature);
-    };
-    auto total_of = [&] {
-      double s = 0.0;
-      for (int k = lane; k < p.chunks; k += 64) s += mass(k);
-      return wave_sum_f64(s);
-    };
-    double total = total_of();
-    if ((minus_q && !(total > kEmptyRest)) || (skip >= 0 && !(total * inv_t > kEmptyRest))) {
-      minus_q = false, skip = -1;
-      total = total_of();
+    int draw = dec.draw;
+    if (draw != kDrawTarget && !(total > kEmptyRest * all)) {
+      draw = kDrawTarget;
+      total = total_of(draw, 0.0);
     }
-    const double threshold = static_cast<double>(p.coins[b * p.coins_stride + p.drafts]) * total;
+    const double threshold = static_cast<double>(coin) * total;
     double before = 0.0;  // of the chunks of the groups of 64 already passed
     int chunk = -1, last_mass = 0;
     double at = INFINITY;
     for (int k0 = 0; k0 < p.chunks && chunk < 0; k0 += 64) {
-      const double m = mass(k0 + lane);
-      double incl = m;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const double o = __shfl_up(incl, d);
-        if (lane >= d) incl += o;
-      }
-      incl += before;
+      const double m = mass_of(k0 + lane, draw, carry);
+      const double incl = wave_scan_f64(m) + before;
       const uint64_t hit = __ballot(m > 0.0 && incl > threshold);
       const uint64_t some = __ballot(m > 0.0);
       if (some) last_mass = k0 + 63 - __clzll(static_cast<long long>(some));
       if (hit) {
         const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
         chunk = k0 + l;
-        at = threshold - (__shfl(incl, l) - __shfl(m, l));
+        at = threshold - (lane_f64(incl, l) - lane_f64(m, l));
       }
-      before = __shfl(incl, 63);
+      before = lane_f64(incl, 63);
     }
     if (chunk < 0) chunk = last_mass;  // (a coin of 1 or more, or a sum that rounds below the threshold: the last entry)
-    if (lane == 0) pick_chunk = chunk, pick_at = at, shared[0] = minus_q, shared[1] = skip;
+    if (lane == 0) pick_chunk = chunk, pick_at = at, pick_draw = draw;
   }
   __syncthreads();
-  const int chunk = pick_chunk;
-  double w[E];
-  weights(chunk, shared[0] != 0, shared[1], w);
-  double mine = 0.0;
+  const int chunk = pick_chunk, draw = pick_draw;
+  const double threshold = pick_at;
+  const int skip = draw == kDrawWithout ? dec.skip : -1;
+  const int at = chunk * kVerifyChunk + tid * E;
+  uint4 t_raw[E / VE], d_raw[E / VE];
 #pragma unroll
-  for (int e = 0; e < E; ++e) mine += w[e];
-  // inclusive scan over the lanes
-  double incl = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double o = __shfl_up(incl, d);
-    if (lane >= d) incl += o;
+  for (int g = 0; g < E / VE; ++g) {
+    t_raw[g] = load_raw<DT>(target_row<DT>(p, b, dec.kept), at + g * VE, p.vocab);
+    if (draw == kDrawRest) d_raw[g] = load_raw<DT>(draft_row<DT>(p, b, dec.kept), at + g * VE, p.vocab);
   }
+  double w[E], mine = 0.0;
+#pragma unroll
+  for (int g = 0; g < E / VE; ++g) {
+    float tv[VE], dv[VE];
+    decode_vec<DT>(t_raw[g], tv);
+    if (draw == kDrawRest) decode_vec<DT>(d_raw[g], dv);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      double& we = w[g * VE + e];
+      we = t_weight(tv[e], table);
+      if (draw == kDrawRest) we = fmax(fma(-rho, d_weight(dv[e], table), we), 0.0);
+      if (at + g * VE + e == skip) we = 0.0;
+      mine += we;
+    }
+  }
+  // inclusive scan over the lanes
+  const double incl = wave_scan_f64(mine);
   if (lane == 63) red[wave] = incl;
   __syncthreads();
   double run = incl - mine;
   for (int v = 0; v < wave; ++v) run += red[v];
-  int first_hit = CHUNK, last_some = -1;
+  int first_hit = kVerifyChunk, last_some = -1;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     run += w[e];
     if (w[e] > 0.0) {
       last_some = tid * E + e;
-      if (run > pick_at && first_hit == CHUNK) first_hit = tid * E + e;
+      if (run > threshold && first_hit == kVerifyChunk) first_hit = tid * E + e;
     }
   }
-  if (first_hit < CHUNK) atomicMin(&found, first_hit);
+  if (first_hit < kVerifyChunk) atomicMin(&found, first_hit);
   if (last_some >= 0) atomicMax(&last, last_some);
   __syncthreads();
-  const int in_chunk = found < CHUNK ? found : last;
-  answer(in_chunk < 0 ? -1 : chunk * CHUNK + in_chunk);
+  const int in_chunk = found < kVerifyChunk ? found : last;
+  answer(in_chunk < 0 ? -1 : chunk * kVerifyChunk + in_chunk);
 }
 
 }  // namespace ets

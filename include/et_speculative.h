@@ -19,9 +19,9 @@
  *           (lowest index wins ties, NaN lowest: the rule of the sampler at temperature 0).  Draft logits
  *           and coins are not read.
  *
- * Probabilities, sums and comparisons are held in 64 bits, so the tokens are those of the formulas in
- * exact arithmetic but for coins within about 1e-11 of a border.  Masked tokens (logit -inf) have
- * probability 0 and are never drawn; top-k and top-p are applied by masking the rows of both models
+ * Decisions are those of 64-bit arithmetic: a token can differ from exact arithmetic only for a coin within
+ * about 1e-10 of a border (of two nearly equal models, whose p - q has a mass of R: 1e-15 / R if that is more).
+ * Masked tokens (logit -inf) have probability 0 and are never drawn; top-k and top-p are applied by masking the rows of both models
  * beforehand.  For T > 0 a row that holds NaN or +inf, or nothing but -inf, has no distribution; neither
  * has any row of a sequence whose temperature is NaN: a sequence that comes to such a row (the target's,
  * or the draft's beside it) gets -1 as its next token there.  A drafted token outside [0, vocab) is
@@ -56,7 +56,7 @@ typedef struct ets_verify_batch {
   int64_t draft_tokens_stride;
   const int32_t* draft_lengths; /* [sequences]: drafts of each sequence, clamped to 0 .. drafts; NULL: all `drafts`.
                                  * Rows, tokens and coins behind a sequence's length are not read. */
-  const float* temperatures;    /* [sequences] or NULL */
+  const float* temperatures;    /* [sequences] or NULL.  Positive ones are taken between 1e-30 and 1e30. */
   const float* coins;           /* [sequences, drafts + 1] uniforms in [0, 1): one per draft, then the draw's */
   int64_t coins_stride;
   int32_t* tokens; /* out: [sequences, drafts + 1]: accepted drafts, the next token, then -1 */

@@ -1,6 +1,5 @@
 """DraftVerifier through the C ABI against the float64 restatement: tokens and counts must be equal.
-(The kernels hold weights and sums to about 1e-13 in 64 bits, so a coin would have to fall within about
-1e-11 of a border for the two to differ: for the draws here a chance below 1e-6 in all.)"""
+(Both work in 64 bits, so a coin would have to fall within about 1e-10 of a border for the two to differ.)"""
 import numpy as np
 import pytest
 import torch
@@ -330,3 +329,38 @@ def test_refusals(dev):
         with pytest.raises(ea.SamplerError):
             call(v, x, **out)
     check(v, x, "the handle still works")
+
+
+@pytest.mark.parametrize("dtype,V", [("f32", 5000), ("bf16", 40000), ("f16", 129)])
+@pytest.mark.parametrize("draft", [True, False])
+def test_coins_next_to_the_border_of_acceptance(dev, dtype, V, draft):
+    """Coins at p / q rounded to fp32 and at its neighbours: closer than fp32 sums could tell, and decided as
+    in 64 bits all the same.  (p / q itself is a real number; a coin lies about 3e-8 of it away.)"""
+    S, K = 96, 3
+    x = problem(97, S, K, V, dtype, dev, draft=draft, temps=(0.6, 1.0, 1.4), sharp=4.0)
+    t, d, tokens = x["target"].float().cpu().numpy(), None if not draft else x["draft"].float().cpu().numpy(), x["tokens"].cpu().numpy()
+    coins, temps = x["coins"].cpu().numpy(), x["temperature"].cpu().numpy()
+    for b in range(S):
+        for i in range(K):
+            p = VO.probabilities(t[b, i], float(temps[b]))[tokens[b, i]]
+            q = VO.probabilities(d[b, i], float(temps[b]))[tokens[b, i]] if draft else 1.0
+            coins[b, i] = np.nextafter(np.float32(p / q), np.float32((0, 2, p / q)[(b + i) % 3]))
+    x["coins"] = torch.from_numpy(coins).to(dev)
+    kept = check(ea.DraftVerifier(V, S, K), x, (dtype, V, draft))
+    assert 0 < kept.sum() < S * K
+
+
+def test_residuals_of_nearly_equal_models(dev):
+    """The draft's rows are the target's but for a few entries: nearly everything cancels in p - q."""
+    S, K, V = 64, 1, 30000
+    x = problem(98, S, K, V, "f32", dev, temps=(0.7, 1.0))
+    g = np.random.default_rng(4)
+    d = x["target"][:, :K].clone()
+    for b in range(S):
+        at = torch.from_numpy(g.integers(0, V, size=5)).to(dev)
+        d[b, 0, at] += torch.from_numpy((10.0 ** -g.integers(1, 4, size=5) * g.choice([-1, 1], size=5)).astype(np.float32)).to(dev)
+    x["draft"] = d
+    x["tokens"][:, 0] = -1  # (always rejected: the draw is from what is left)
+    check(ea.DraftVerifier(V, S, K), x, "nearly equal")
+    x["draft"] = x["target"][:, :K] + 3.0  # all but the same distribution: what is left is fp32's rounding of the shift
+    check(ea.DraftVerifier(V, S, K), x, "shifted")
