@@ -192,6 +192,7 @@ ets_status ets_logit_head_logits(ets_logit_head* h, const void* d_hidden, int32_
   p.blocks = static_cast<const ets::u32x4*>(h->d_blocks);
   p.scales = h->d_scales;
   p.zeros = h->d_zeros;
+  p.scale_bytes = h->form.scale_bytes;
   p.scale_is_bf16 = h->scale_is_bf16;
   p.tiles = h->tiles;
   p.chunks = h->chunks;

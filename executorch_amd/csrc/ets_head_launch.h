@@ -24,8 +24,27 @@ hipError_t launch_head(const ets::HeadParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <int XT, int GPC, int MT, int NT, int WV, int WK>
+hipError_t launch_tiles(const ets::HeadParams& p, hipStream_t stream) {
+  const int64_t vocab_blocks = (p.tiles + WV * NT - 1) / (WV * NT), row_blocks = (p.rows + 16 * MT - 1) / (16 * MT);
+  hipLaunchKernelGGL((ets::head_tile_kernel<XT, GPC, MT, NT, WV, WK>), dim3(static_cast<uint32_t>((vocab_blocks + 7) / 8 * 8 * row_blocks)),
+                     dim3(64 * WV * WK), 0, stream, p);
+  return hipGetLastError();
+}
+
+template <int XT, int GPC, int MT>
+hipError_t launch_tiles(const ets::HeadParams& p, hipStream_t stream) {
+  // 256 vocabulary entries a workgroup where that makes at least one for each of the 256 CUs; otherwise 128, with twice
+  // the waves behind each other along the columns.
+  return p.tiles >= 256 * 16 ? launch_tiles<XT, GPC, MT, 4, 4, 1>(p, stream) : launch_tiles<XT, GPC, MT, 2, 4, 2>(p, stream);
+}
+
 template <int XT, int GPC>
 hipError_t launch_head(const ets::HeadParams& p, const HeadForm& f, hipStream_t stream) {
+  if (p.rows > 16) {
+    if (p.rows <= 32 || XT == ets::kDtypeFloat) return launch_tiles<XT, GPC, 2>(p, stream);
+    return launch_tiles<XT, GPC, XT == ets::kDtypeFloat ? 2 : 4>(p, stream);
+  }
   if (f.scale_bytes == 4) return f.zeros ? launch_head<XT, GPC, 4, true>(p, stream) : launch_head<XT, GPC, 4, false>(p, stream);
   return f.zeros ? launch_head<XT, GPC, 2, true>(p, stream) : launch_head<XT, GPC, 2, false>(p, stream);
 }
