@@ -13,15 +13,14 @@ namespace ets {
 // ---- layout -------------------------------------------------------------------------------------
 // One lane per dword of the blocks.  Columns and rows that do not exist hold n = 8, the weight 0.
 __global__ void __launch_bounds__(kHeadBlock)
-head_layout_kernel(const uint8_t* packed, int64_t stride, int32_t vocab, int32_t hidden, int32_t chunks, int64_t dwords,
+head_layout_kernel(const uint8_t* packed, int64_t stride, int32_t vocab, int32_t hidden, int32_t tiles, int64_t dwords,
                    uint32_t* blocks) {
   for (int64_t d = static_cast<int64_t>(blockIdx.x) * kHeadBlock + threadIdx.x; d < dwords;
        d += static_cast<int64_t>(gridDim.x) * kHeadBlock) {
     const int t = static_cast<int>(d & 3), lane = static_cast<int>((d >> 2) & 63);
-    const int64_t block = d >> 8, tile = block / chunks;
-    const int chunk = static_cast<int>(block - tile * chunks);
-    const int64_t v = tile * kTileRows + (lane & 15);
-    const int k = chunk * kChunkCols + 32 * t + 8 * (lane >> 4);
+    const int64_t block = d >> 8, chunk = block / tiles;
+    const int64_t v = (block - chunk * tiles) * kTileRows + (lane & 15);
+    const int k = static_cast<int>(chunk) * kChunkCols + 32 * t + 8 * (lane >> 4);
     uint32_t w = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -36,14 +35,13 @@ head_layout_kernel(const uint8_t* packed, int64_t stride, int32_t vocab, int32_t
 // One lane per scale (or zero) of the layout; groups and rows that do not exist hold 0.
 template <typename T>
 __global__ void __launch_bounds__(kHeadBlock)
-head_scales_kernel(const T* scales, int32_t vocab, int32_t groups, int32_t per_chunk, int64_t per_tile, int64_t count, T* out) {
+head_scales_kernel(const T* scales, int32_t vocab, int32_t groups, int32_t per_chunk, int32_t tiles, int64_t count, T* out) {
   for (int64_t d = static_cast<int64_t>(blockIdx.x) * kHeadBlock + threadIdx.x; d < count;
        d += static_cast<int64_t>(gridDim.x) * kHeadBlock) {
-    const int64_t tile = d / per_tile;
-    const int64_t in_tile = d - tile * per_tile;
-    const int64_t of = in_tile / (kTileRows * per_chunk);  // chunk, or group of 128 columns and more
-    const int rest = static_cast<int>(in_tile - of * (kTileRows * per_chunk));
-    const int64_t v = tile * kTileRows + rest / per_chunk, group = of * per_chunk + rest % per_chunk;
+    const int64_t of_tile = d / (kTileRows * per_chunk);
+    const int rest = static_cast<int>(d - of_tile * (kTileRows * per_chunk));
+    const int64_t of = of_tile / tiles;  // chunk, or group of 128 columns and more
+    const int64_t v = (of_tile - of * tiles) * kTileRows + rest / per_chunk, group = of * per_chunk + rest % per_chunk;
     out[d] = (v < vocab && group < groups) ? scales[v * groups + group] : static_cast<T>(0);
   }
 }
@@ -59,6 +57,8 @@ struct ets_logit_head {
   void* d_blocks = nullptr;
   void* d_scales = nullptr;
   void* d_zeros = nullptr;
+  void* d_units = nullptr;  // hidden states of a call with more than 16 rows, laid out as operands
+  void* d_sums = nullptr;   // and their sums over each group
   char last_error[256] = "";
 };
 
@@ -134,13 +134,12 @@ ets_status ets_logit_head_create(int32_t vocab_size, int32_t hidden_size, int32_
   e = hipMalloc(&h->d_blocks, dwords * 4);
   if (e != hipSuccess) return bail(e, "ets_logit_head_create: hipMalloc(weights)");
   hipLaunchKernelGGL(ets::head_layout_kernel, dim3(layout_grid(dwords)), dim3(ets::kHeadBlock), 0, stream,
-                     static_cast<const uint8_t*>(d_packed), packed_stride, vocab_size, hidden_size, h->chunks, dwords,
+                     static_cast<const uint8_t*>(d_packed), packed_stride, vocab_size, hidden_size, h->tiles, dwords,
                      static_cast<uint32_t*>(h->d_blocks));
   e = hipGetLastError();
   if (e != hipSuccess) return bail(e, "ets_logit_head_create: launch");
   const int32_t per_chunk = h->form.groups_per_chunk;
-  const int64_t per_tile = static_cast<int64_t>(ets::kTileRows) * (per_chunk > 1 ? h->chunks * per_chunk : groups);
-  const int64_t count = per_tile * h->tiles;
+  const int64_t count = static_cast<int64_t>(ets::kTileRows) * h->tiles * (per_chunk > 1 ? h->chunks * per_chunk : groups);
   for (int k = 0; k < (d_zeros ? 2 : 1); ++k) {
     void** dst = k ? &h->d_zeros : &h->d_scales;
     const void* src = k ? d_zeros : d_scales;
@@ -148,14 +147,19 @@ ets_status ets_logit_head_create(int32_t vocab_size, int32_t hidden_size, int32_
     if (e != hipSuccess) return bail(e, "ets_logit_head_create: hipMalloc(scales)");
     if (scale_bytes == 4) {
       hipLaunchKernelGGL((ets::head_scales_kernel<uint32_t>), dim3(layout_grid(count)), dim3(ets::kHeadBlock), 0, stream,
-                         static_cast<const uint32_t*>(src), vocab_size, groups, per_chunk, per_tile, count, static_cast<uint32_t*>(*dst));
+                         static_cast<const uint32_t*>(src), vocab_size, groups, per_chunk, h->tiles, count, static_cast<uint32_t*>(*dst));
     } else {
       hipLaunchKernelGGL((ets::head_scales_kernel<uint16_t>), dim3(layout_grid(count)), dim3(ets::kHeadBlock), 0, stream,
-                         static_cast<const uint16_t*>(src), vocab_size, groups, per_chunk, per_tile, count, static_cast<uint16_t*>(*dst));
+                         static_cast<const uint16_t*>(src), vocab_size, groups, per_chunk, h->tiles, count, static_cast<uint16_t*>(*dst));
     }
     e = hipGetLastError();
     if (e != hipSuccess) return bail(e, "ets_logit_head_create: launch");
   }
+  const size_t work_chunks = static_cast<size_t>(ets::padded_chunks(h->chunks));
+  e = hipMalloc(&h->d_units, ets_host::kWorkTiles * work_chunks * 4096);
+  if (e != hipSuccess) return bail(e, "ets_logit_head_create: hipMalloc(work buffer)");
+  e = hipMalloc(&h->d_sums, ets_host::kWorkTiles * work_chunks * per_chunk * 64);
+  if (e != hipSuccess) return bail(e, "ets_logit_head_create: hipMalloc(work buffer)");
   e = hipStreamSynchronize(stream);
   if (e != hipSuccess) return bail(e, "ets_logit_head_create: hipStreamSynchronize");
   *out = h;
@@ -169,6 +173,8 @@ ets_status ets_logit_head_destroy(ets_logit_head* h) {
     (void)hipFree(h->d_blocks);
     (void)hipFree(h->d_scales);
     (void)hipFree(h->d_zeros);
+    (void)hipFree(h->d_units);
+    (void)hipFree(h->d_sums);
   }
   delete h;
   return ETS_OK;
@@ -198,9 +204,12 @@ ets_status ets_logit_head_logits(ets_logit_head* h, const void* d_hidden, int32_
   p.chunks = h->chunks;
   p.chunks_per_group = h->chunks_per_group;
   p.groups = h->groups;
+  p.group_magic = static_cast<uint32_t>(((int64_t{1} << 32) + h->chunks_per_group - 1) / h->chunks_per_group);  // (not read for 1)
   p.vocab = h->vocab;
   p.hidden = h->hidden;
   p.rows = rows;
+  p.units = static_cast<const ets::u32x4*>(h->d_units);
+  p.sums = static_cast<const ets::f32x4*>(h->d_sums);
   p.x = d_hidden;
   p.x_stride = hidden_stride;
   p.out = d_logits;

@@ -12,6 +12,9 @@ struct HeadForm {
   bool zeros;
 };
 
+// 16-row tiles (of 16-bit parts) that the work buffer of more than 16 rows holds: calls with more go through it in turns.
+constexpr int kWorkTiles = 32;
+
 hipError_t launch_head_f32(const ets::HeadParams& p, const HeadForm& f, hipStream_t stream);
 hipError_t launch_head_f16(const ets::HeadParams& p, const HeadForm& f, hipStream_t stream);
 hipError_t launch_head_bf16(const ets::HeadParams& p, const HeadForm& f, hipStream_t stream);
@@ -24,29 +27,50 @@ hipError_t launch_head(const ets::HeadParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int XT, int GPC, int MT, int NT, int WV, int WK>
+template <int XT, int GPC, int SB, bool ZEROS, int MT, int NT, int WV, int WK>
 hipError_t launch_tiles(const ets::HeadParams& p, hipStream_t stream) {
   const int64_t vocab_blocks = (p.tiles + WV * NT - 1) / (WV * NT), row_blocks = (p.rows + 16 * MT - 1) / (16 * MT);
-  hipLaunchKernelGGL((ets::head_tile_kernel<XT, GPC, MT, NT, WV, WK>), dim3(static_cast<uint32_t>((vocab_blocks + 7) / 8 * 8 * row_blocks)),
-                     dim3(64 * WV * WK), 0, stream, p);
+  hipLaunchKernelGGL((ets::head_tile_kernel<XT, GPC, SB, ZEROS, MT, NT, WV, WK>),
+                     dim3(static_cast<uint32_t>((vocab_blocks + 7) / 8 * 8 * row_blocks)), dim3(64 * WV * WK), 0, stream, p);
   return hipGetLastError();
 }
 
-template <int XT, int GPC, int MT>
+template <int XT, int GPC, int SB, bool ZEROS, int MT>
 hipError_t launch_tiles(const ets::HeadParams& p, hipStream_t stream) {
-  // 256 vocabulary entries a workgroup where that makes at least one for each of the 256 CUs; otherwise 128, with twice
-  // the waves behind each other along the columns.
-  return p.tiles >= 256 * 16 ? launch_tiles<XT, GPC, MT, 4, 4, 1>(p, stream) : launch_tiles<XT, GPC, MT, 2, 4, 2>(p, stream);
+  // 512 vocabulary entries a workgroup where that makes at least one for nearly each of the 256 CUs; otherwise 128, with
+  // two waves behind each other along the columns.
+  return p.tiles >= 240 * 32 ? launch_tiles<XT, GPC, SB, ZEROS, MT, 4, 8, 1>(p, stream) : launch_tiles<XT, GPC, SB, ZEROS, MT, 2, 4, 2>(p, stream);
+}
+
+template <int XT, int GPC, int SB, bool ZEROS>
+hipError_t launch_head_rows(const ets::HeadParams& whole, hipStream_t stream) {
+  if (whole.rows <= 16) return launch_head<XT, GPC, SB, ZEROS>(whole, stream);
+  constexpr int kRowsAtOnce = kWorkTiles / ets::Parts<XT>::value / 2 * 2 * 16;  // as the work buffer holds
+  const int32_t chunks = ets::padded_chunks(whole.chunks);
+  for (int32_t row = 0; row < whole.rows; row += kRowsAtOnce) {
+    ets::HeadParams p = whole;
+    p.rows = whole.rows - row < kRowsAtOnce ? whole.rows - row : kRowsAtOnce;
+    p.out = static_cast<char*>(whole.out) + row * whole.out_stride * (whole.out_dtype == ets::kDtypeFloat ? 4 : 2);
+    hipLaunchKernelGGL((ets::head_rows_kernel<XT, GPC>), dim3(chunks, (p.rows + 15) / 16), dim3(ets::kHeadBlock), 0, stream,
+                       static_cast<const char*>(whole.x) + row * whole.x_stride * ets::ElemSize<XT>::value, p.x_stride, p.rows, p.hidden,
+                       const_cast<ets::u32x4*>(p.units), const_cast<float*>(reinterpret_cast<const float*>(p.sums)));
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    e = p.rows <= 32 || XT == ets::kDtypeFloat ? launch_tiles<XT, GPC, SB, ZEROS, 2>(p, stream)
+                                               : launch_tiles<XT, GPC, SB, ZEROS, XT == ets::kDtypeFloat ? 2 : 4>(p, stream);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+template <int XT, int GPC, bool ZEROS>
+hipError_t launch_head(const ets::HeadParams& p, const HeadForm& f, hipStream_t stream) {
+  return f.scale_bytes == 4 ? launch_head_rows<XT, GPC, 4, ZEROS>(p, stream) : launch_head_rows<XT, GPC, 2, ZEROS>(p, stream);
 }
 
 template <int XT, int GPC>
 hipError_t launch_head(const ets::HeadParams& p, const HeadForm& f, hipStream_t stream) {
-  if (p.rows > 16) {
-    if (p.rows <= 32 || XT == ets::kDtypeFloat) return launch_tiles<XT, GPC, 2>(p, stream);
-    return launch_tiles<XT, GPC, XT == ets::kDtypeFloat ? 2 : 4>(p, stream);
-  }
-  if (f.scale_bytes == 4) return f.zeros ? launch_head<XT, GPC, 4, true>(p, stream) : launch_head<XT, GPC, 4, false>(p, stream);
-  return f.zeros ? launch_head<XT, GPC, 2, true>(p, stream) : launch_head<XT, GPC, 2, false>(p, stream);
+  return f.zeros ? launch_head<XT, GPC, true>(p, f, stream) : launch_head<XT, GPC, false>(p, f, stream);
 }
 
 template <int XT>

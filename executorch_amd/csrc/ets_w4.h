@@ -12,7 +12,9 @@
 // Weight layout: blocks of 16 vocabulary rows x 128 columns, 1 KiB, the 16 bytes of a lane next to each
 // other: lane (q, n) = 16 q + n holds row n of the block, its dword t the columns 32 t + 8 q + 0..7 (operand
 // B of the t-th 16x16x32 product), the column 8 q + 2 i + h at bits 16 h + 4 i.  A wave reads a block with
-// one 16-byte load per lane.
+// one 16-byte load per lane.  The blocks of one chunk of columns are next to each other: workgroups that walk
+// along the columns side by side then read one contiguous stretch of memory at a time, where blocks in row order
+// (32 KiB apart at 4096 columns) would have all of them at the same memory channels (64 rows: 134 us).
 #pragma once
 
 #include "ets_device.h"
@@ -29,15 +31,18 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct HeadParams {
-  const u32x4* blocks;  // [tiles, chunks, 64]
-  const void* scales;   // [tiles, chunks, 16, groups per chunk], or [tiles, groups, 16] for groups of 128 columns and more
+  const u32x4* blocks;  // [chunks, tiles, 64]
+  const void* scales;   // [chunks, tiles, 16, groups per chunk], or [groups, tiles, 16] for groups of 128 columns and more
   const void* zeros;    // the same, or null
   int32_t scale_bytes;    // 4 (fp32) or 2
   int32_t scale_is_bf16;  // of 16-bit scales: bf16, else fp16
   int32_t tiles, chunks, chunks_per_group, groups;  // (the last two for groups of 128 columns and more)
+  uint32_t group_magic;   // ceil(2^32 / chunks_per_group): the upper word of chunk x group_magic is the chunk's group
   int32_t vocab, hidden, rows;
-  const void* x;
+  const void* x;          // of head_stream
   int64_t x_stride;
+  const u32x4* units;     // of head_tile: what head_rows has written
+  const f32x4* sums;
   void* out;
   int64_t out_stride;
   int32_t out_dtype;
@@ -63,15 +68,22 @@ struct Matrix<kDtypeHalf> {
   }
 };
 
-// Eight packed weights as an operand: 16 + n each.
+// Eight packed weights as an operand: 16 + n each.  `base` is Matrix::kBase from base_in_register(): the and-or is one
+// instruction only if one of its constants is in a vector register.
 template <int XT>
-__device__ __forceinline__ u32x4 unpack(uint32_t w) {
+__device__ __forceinline__ uint32_t base_in_register() {
+  uint32_t base = Matrix<XT>::kBase;
+  asm("" : "+v"(base));
+  return base;
+}
+template <int XT>
+__device__ __forceinline__ u32x4 unpack(uint32_t w, uint32_t base) {
   using M = Matrix<XT>;
   u32x4 b;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int shift = 4 * i - M::kTop;
-    b[i] = ((shift < 0 ? w << -shift : w >> shift) & M::kMask) | M::kBase;
+    b[i] = ((shift < 0 ? w << -shift : w >> shift) & M::kMask) | base;
   }
   return b;
 }
@@ -95,26 +107,29 @@ struct RawX {  // eight columns of x as they are in memory
 
 // Columns [k, k + 8) of a row; columns at `hidden` and behind, and rows that do not exist, read as 0.
 template <int XT>
-__device__ __forceinline__ RawX<XT> load_raw_x(const void* row, int k, int hidden, bool exists) {
+__device__ __forceinline__ RawX<XT> load_whole_x(const char* at) {
+  RawX<XT> out;
+  if (XT == kDtypeFloat) {
+    const LooseFloats r = *reinterpret_cast<const LooseFloats*>(at);
+    __builtin_memcpy(out.v, &r, 32);
+  } else {
+    const LooseHalves r = *reinterpret_cast<const LooseHalves*>(at);
+    __builtin_memcpy(out.v, &r, 16);
+  }
+  return out;
+}
+template <int XT>
+__device__ __forceinline__ RawX<XT> load_raw_x(const char* row, int k, int hidden, bool exists) {
   RawX<XT> out = {};
   if (!exists) return out;
-  if (k + 8 <= hidden) {
-    if (XT == kDtypeFloat) {
-      const LooseFloats r = *reinterpret_cast<const LooseFloats*>(static_cast<const float*>(row) + k);
-      __builtin_memcpy(out.v, &r, 32);
-    } else {
-      const LooseHalves r = *reinterpret_cast<const LooseHalves*>(static_cast<const uint16_t*>(row) + k);
-      __builtin_memcpy(out.v, &r, 16);
-    }
-    return out;
-  }
+  if (k + 8 <= hidden) return load_whole_x<XT>(row + static_cast<int64_t>(k) * ElemSize<XT>::value);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     if (k + j < hidden) {
       if (XT == kDtypeFloat) {
-        out.v[j >> 2][j & 3] = static_cast<const uint32_t*>(row)[k + j];
+        out.v[j >> 2][j & 3] = reinterpret_cast<const uint32_t*>(row)[k + j];
       } else {
-        out.v[0][j >> 1] |= static_cast<uint32_t>(static_cast<const uint16_t*>(row)[k + j]) << (16 * (j & 1));
+        out.v[0][j >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[k + j]) << (16 * (j & 1));
       }
     }
   }
@@ -146,11 +161,15 @@ __device__ __forceinline__ void split_x(const RawX<XT>& x, u32x4* part) {
   }
 }
 
+// The group of a chunk, for groups of 128 columns and more.  (Exact: chunk and chunks_per_group are at most 2^13.)
+__device__ __forceinline__ int chunk_group(const HeadParams& p, int chunk) {
+  return p.chunks_per_group == 1 ? chunk : static_cast<int>(__umulhi(static_cast<uint32_t>(chunk), p.group_magic));
+}
+
 // The scales (or zeros) of this lane's vocabulary row for the GPC groups of a chunk.
 template <int GPC, int SB>
 __device__ __forceinline__ void load_scales(const void* base, const HeadParams& p, int tile, int chunk, int n, float* s) {
-  const int64_t at = GPC > 1 ? ((static_cast<int64_t>(tile) * p.chunks + chunk) * kTileRows + n) * GPC
-                             : (static_cast<int64_t>(tile) * p.groups + chunk / p.chunks_per_group) * kTileRows + n;
+  const int64_t at = ((static_cast<int64_t>(GPC > 1 ? chunk : chunk_group(p, chunk)) * p.tiles + tile) * kTileRows + n) * GPC;
   if (SB == 4) {
     struct alignas(4 * GPC) Raw { float f[GPC]; };
     const Raw r = *reinterpret_cast<const Raw*>(static_cast<const float*>(base) + at);
@@ -209,11 +228,12 @@ head_stream_kernel(const HeadParams p) {
   using M = Matrix<XT>;
   constexpr int P = Parts<XT>::value, kWavesHere = kHeadBlock / 64, kSteps = 4 / GPC;  // products per group of a chunk
   __shared__ float red[kWavesHere][NT][64 * 4];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 15, q = lane >> 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, q = lane >> 4;
   const int tile0 = blockIdx.x * NT, m0 = blockIdx.y * 16;
   const bool exists = m0 + n < p.rows;
   const char* x_row = static_cast<const char*>(p.x) + (exists ? m0 + n : 0) * p.x_stride * ElemSize<XT>::value;
   const u32x4 minus24 = {M::kMinus24, M::kMinus24, M::kMinus24, M::kMinus24}, one = {M::kOne, M::kOne, M::kOne, M::kOne};
+  const uint32_t unpack_base = base_in_register<XT>();
   f32x4 total[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) total[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -224,7 +244,7 @@ head_stream_kernel(const HeadParams p) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int tile = min(tile0 + i, p.tiles - 1);  // (tiles behind the last one are computed again and not stored)
-      w[i] = p.blocks[(static_cast<int64_t>(tile) * p.chunks + chunk) * 64 + lane];
+      w[i] = p.blocks[(static_cast<int64_t>(chunk) * p.tiles + tile) * 64 + lane];
       load_scales<GPC, SB>(p.scales, p, tile, chunk, n, s[i]);
       if (ZEROS) load_scales<GPC, SB>(p.zeros, p, tile, chunk, n, z[i]);
     }
@@ -247,7 +267,7 @@ head_stream_kernel(const HeadParams p) {
         f32x4 acc = base;
 #pragma unroll
         for (int t = g * kSteps; t < (g + 1) * kSteps; ++t) {
-          const u32x4 b = unpack<XT>(w[i][t]);
+          const u32x4 b = unpack<XT>(w[i][t], unpack_base);
 #pragma unroll
           for (int k = 0; k < P; ++k) acc = M::product(x[t][k], b, acc);
         }
@@ -275,13 +295,16 @@ head_stream_kernel(const HeadParams p) {
 }
 
 // ---- the product, many rows ---------------------------------------------------------------------
-// A workgroup makes (16 MT) rows x (16 NT WV) vocabulary entries: WV waves next to each other along the
-// vocabulary, WK of them behind each other along the columns (each takes every WK-th chunk; their sums are
-// added up in the end).  x goes through LDS, where all waves read it as operand A; a wave's weights go from
-// memory to its registers, unpacked there once for all of its rows.  While one chunk is multiplied the next
-// one's weights and hidden states are on their way; one barrier per chunk.
-// In LDS the 16 bytes of row m, columns 32 t + 8 q + 0..7, lie at 16-byte unit 64 t + 16 q + (m ^ (4 t + q)) of their
-// 16 rows: a wave's read of an operand and its write of four rows both touch every bank once.
+// head_rows writes the hidden states as operand A into the handle's work buffer, head_tile multiplies them: a
+// workgroup makes (16 MT) rows x (16 NT WV) vocabulary entries, WV waves next to each other along the
+// vocabulary, WK behind each other along the columns (each takes every WK-th chunk; their sums are added
+// up in the end).  x goes through LDS, where all waves read it; a wave's weights go from memory to its
+// registers, unpacked there once for all of its rows.
+//
+// Work buffer: per 16 rows and chunk of columns, and part of x, 256 units of 16 bytes: row m, columns
+// 32 t + 8 q + 0..7 at unit 16 (4 t + q) + m, so that a wave reads an operand as one contiguous KiB; rows and
+// columns that do not exist are 0.  Behind all of these, per 16 rows and chunk, -24 times the rows' sums of x
+// over each group of the chunk: what the accumulators start from.
 // -24 times the sum of the eight columns.
 template <int XT>
 __device__ __forceinline__ float minus24_sum(const RawX<XT>& x) {
@@ -310,49 +333,75 @@ __device__ __forceinline__ float dpp_add(float v) {
   return v + __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), CTRL, 0xf, 0xf, false));
 }
 
-// The scales of this lane's vocabulary row for a chunk's groups, as they are in memory (4 words at most).
-template <int GPC>
-struct RawScales {
-  uint32_t v[GPC];
-};
-template <int GPC>
-__device__ __forceinline__ RawScales<GPC> load_raw_scales(const void* base, const HeadParams& p, int tile, int chunk, int n) {
-  const int64_t at = GPC > 1 ? ((static_cast<int64_t>(tile) * p.chunks + chunk) * kTileRows + n) * GPC
-                             : (static_cast<int64_t>(tile) * p.groups + chunk / p.chunks_per_group) * kTileRows + n;
-  RawScales<GPC> r = {};
-  if (p.scale_bytes == 4) {
-    r = *reinterpret_cast<const RawScales<GPC>*>(static_cast<const uint32_t*>(base) + at);
-  } else if (GPC == 1) {
-    r.v[0] = static_cast<const uint16_t*>(base)[at];
-  } else {
-    struct alignas(GPC > 1 ? 2 * GPC : 4) Pairs { uint32_t v[GPC > 1 ? GPC / 2 : 1]; };
-    const Pairs h = *reinterpret_cast<const Pairs*>(static_cast<const uint16_t*>(base) + at);
+
+// Chunks of the work buffer: whole rounds of head_tile, whatever its WK; those too many are 0 as well.
+constexpr int kChunkRound = 8;
+__host__ __device__ __forceinline__ int padded_chunks(int chunks) { return (chunks + kChunkRound - 1) / kChunkRound * kChunkRound; }
+
+template <int XT, int GPC>
+__global__ void __launch_bounds__(kHeadBlock)
+head_rows_kernel(const void* x, int64_t x_stride, int32_t rows, int32_t hidden, u32x4* units, float* sums) {
+  constexpr int P = Parts<XT>::value;
+  const int slot = threadIdx.x & 15, in_tile = threadIdx.x >> 4, chunk = blockIdx.x, m = blockIdx.y * 16 + in_tile;
+  const bool exists = m < rows;
+  const char* row = static_cast<const char*>(x) + (exists ? m : 0) * x_stride * ElemSize<XT>::value;
+  const RawX<XT> raw = load_raw_x<XT>(row, chunk * kChunkCols + 8 * slot, hidden, exists);
+  u32x4 part[P];
+  split_x<XT>(raw, part);
+  const int64_t block = static_cast<int64_t>(blockIdx.y) * gridDim.x + chunk;
 #pragma unroll
-    for (int i = 0; i < GPC / 2; ++i) r.v[i] = h.v[i];
+  for (int c = 0; c < P; ++c) units[(block * P + c) * 256 + slot * 16 + in_tile] = part[c];
+  float s = minus24_sum<XT>(raw);  // the 16 lanes of a row hold its chunk
+  s = dpp_add<0xb1>(s);
+  s = dpp_add<0x4e>(s);
+  if (GPC <= 2) s = dpp_add<0x141>(s);
+  if (GPC == 1) s = dpp_add<0x140>(s);
+  if (slot % (16 / GPC) == 0) sums[(block * GPC + slot / (16 / GPC)) * 16 + in_tile] = s;
+}
+
+// The scales of a vocabulary row for a chunk's groups, as they are in memory: GPC of SB bytes.  `there`: all bits, or
+// none, which makes it 0.
+template <int GPC, int SB>
+struct RawScales {
+  uint32_t v[GPC * SB > 4 ? GPC * SB / 4 : 1];
+};
+template <int GPC, int SB>
+__device__ __forceinline__ RawScales<GPC, SB> load_raw_scales(const char* at) {
+  RawScales<GPC, SB> r;
+  if (GPC * SB == 2) {
+    r.v[0] = *reinterpret_cast<const uint16_t*>(at);
+  } else {
+    struct alignas(GPC * SB > 2 ? GPC * SB : 4) Words { uint32_t v[GPC * SB > 4 ? GPC * SB / 4 : 1]; };
+    const Words w = *reinterpret_cast<const Words*>(at);
+#pragma unroll
+    for (int i = 0; i < (GPC * SB > 4 ? GPC * SB / 4 : 1); ++i) r.v[i] = w.v[i];
   }
   return r;
 }
-template <int GPC>
-__device__ __forceinline__ float scale_of(const RawScales<GPC>& r, const HeadParams& p, int g) {
-  if (p.scale_bytes == 4) return __uint_as_float(r.v[g]);
-  const uint32_t h = GPC == 1 ? r.v[0] : (g & 1 ? r.v[g >> 1] >> 16 : r.v[g >> 1] & 0xffffu);
-  return p.scale_is_bf16 ? __uint_as_float(h << 16) : half_bits_to_float(h);
+template <int GPC, int SB>
+__device__ __forceinline__ float scale_of(const RawScales<GPC, SB>& r, const HeadParams& p, int g, uint32_t there) {
+  if (SB == 4) return __uint_as_float(r.v[SB == 4 ? g : 0] & there);
+  const uint32_t pair = r.v[SB == 4 ? 0 : g >> 1], h = g & 1 ? pair >> 16 : pair & 0xffffu;
+  // (chosen by bits: a branch would wait for all loads in flight)
+  const uint32_t bf16 = 0u - static_cast<uint32_t>(p.scale_is_bf16);
+  return __uint_as_float((h << 16 & bf16 & there) | (__float_as_uint(half_bits_to_float(h)) & ~bf16 & there));
 }
 
-template <int XT, int GPC, int MT, int NT, int WV, int WK>
+template <int XT, int GPC, int SB, bool ZEROS, int MT, int NT, int WV, int WK>
 __global__ void __launch_bounds__(64 * WV * WK, 2)
 head_tile_kernel(const HeadParams p) {
   using M = Matrix<XT>;
   constexpr int P = Parts<XT>::value, kSteps = 4 / GPC, kLanes = 64 * WV * WK, kRows = 16 * MT;
-  constexpr int kPieces = WK * kRows * 16 / kLanes;  // of eight columns, per lane and step
-  static_assert(WK * kRows * 16 % kLanes == 0, "");
-  constexpr int kUnits = WK * P * MT * 256;          // of 16 bytes, per buffer
-  constexpr int kOut = WK * WV * 16 * NT * 16;       // floats of 16 rows of the result
+  constexpr int kUnits = WK * P * MT * 256;  // of x per step
+  constexpr int kCopies = kUnits / kLanes;   // of them per lane
+  constexpr int kSums = WK * MT * GPC * 4;   // quadruples of row sums per step
+  static_assert(kUnits % kLanes == 0 && kSums <= kLanes, "");
+  constexpr int kOut = WK * WV * 16 * NT * 16;  // floats of 16 rows of the result
   constexpr int kBytes = 2 * kUnits * 16 > kOut * 4 ? 2 * kUnits * 16 : kOut * 4;
   __shared__ __attribute__((aligned(16))) char lds[kBytes];
-  __shared__ float base_lds[2][WK][GPC][kRows];
+  __shared__ f32x4 sums_lds[2][kSums];
   u32x4* units = reinterpret_cast<u32x4*>(lds);
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 15, q = lane >> 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, q = lane >> 4;
   const int wv = wave % WV, wk = wave / WV;
   // Workgroups of one XCD (every eighth) take the row blocks of a vocabulary block one after the other, so that its
   // weights come from memory once.
@@ -360,114 +409,137 @@ head_tile_kernel(const HeadParams p) {
   const int at = blockIdx.x >> 3, vocab_block = at / row_blocks * 8 + (blockIdx.x & 7), row_block = at % row_blocks;
   if (vocab_block >= vocab_blocks) return;
   const int m0 = row_block * kRows, tile0 = (vocab_block * WV + wv) * NT;
+  const int row_tiles = (p.rows + 15) / 16;
 
-  RawX<XT> x_raw[kPieces];
-  u32x4 w_raw[NT];
-  RawScales<GPC> s_raw[NT], z_raw[NT];
+  // Weights and scales run kAhead steps ahead, hidden states one: their loads are issued first in a step, so that waiting
+  // for them does not wait for the weights behind them.  Each slot of the ring has registers of its own (the loop is
+  // unrolled kAhead times): a copy would wait for what is copied.
+  constexpr int kAhead = 2;
+  static_assert(kAhead % 2 == 0 && kChunkRound % (kAhead * WK) == 0, "the buffers in LDS alternate with the slots; whole rounds");
+  u32x4 x_raw[kCopies], w_raw[kAhead][NT];
+  f32x4 sums_raw;
+  RawScales<GPC, SB> s_raw[kAhead][NT], z_raw[kAhead][NT];
+  // Unit u of a step: chunk u / (256 P MT) of it, 16-row tile u / (256 P) % MT (of those that do not exist the last one).
+  // Everything but the lane's offset is the same in every lane of a wave.
+  const int work_chunks = padded_chunks(p.chunks);
+  const int sum_u = min(tid, kSums - 1);
+  const uint32_t sum_at = (static_cast<uint32_t>(min(row_block * MT + sum_u / (GPC * 4) % MT, row_tiles - 1) * work_chunks +
+                                                 sum_u / (GPC * 4 * MT)) * (GPC * 4) + sum_u % (GPC * 4)) * 16;
   auto load_step_x = [&](int step) {
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int piece = i * kLanes + tid, slot = piece & 15, row = (piece >> 4) % kRows, chunk = step * WK + piece / (16 * kRows);
-      const int m = m0 + row;
-      const char* x_row = static_cast<const char*>(p.x) + (m < p.rows ? m : 0) * p.x_stride * ElemSize<XT>::value;
-      x_raw[i] = load_raw_x<XT>(x_row, chunk * kChunkCols + 8 * slot, p.hidden, m < p.rows);
+    for (int i = 0; i < kCopies; ++i) {
+      const int u = i * kLanes + wave * 64, tile = min(row_block * MT + u / (256 * P) % MT, row_tiles - 1);
+      const int64_t unit = (static_cast<int64_t>(tile) * work_chunks + step * WK + u / (256 * P * MT)) * (256 * P) + u % (256 * P);
+      x_raw[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p.units) + unit * 16 + static_cast<uint32_t>(lane * 16));
     }
-  };
-  auto load_step_w = [&](int step) {
-    const int chunk = min(step * WK + wk, p.chunks - 1);
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int tile = min(tile0 + i, p.tiles - 1);
-      w_raw[i] = p.blocks[(static_cast<int64_t>(tile) * p.chunks + chunk) * 64 + lane];
-      s_raw[i] = load_raw_scales<GPC>(p.scales, p, tile, chunk, n);
-      if (p.zeros) z_raw[i] = load_raw_scales<GPC>(p.zeros, p, tile, chunk, n);
-    }
+    sums_raw = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(p.sums) + static_cast<int64_t>(step) * (WK * GPC * 64) + sum_at);
   };
   auto store_step_x = [&](int buffer) {
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int piece = i * kLanes + tid, slot = piece & 15, row = (piece >> 4) % kRows, k = piece / (16 * kRows);
-      u32x4 part[P];
-      split_x<XT>(x_raw[i], part);
+    for (int i = 0; i < kCopies; ++i) units[buffer * kUnits + i * kLanes + tid] = x_raw[i];
+    sums_lds[buffer][sum_u] = sums_raw;
+  };
+  // (all of these offsets but the lane's are the same in every lane)
+  auto load_step_w = [&](int step, int slot) {
+    const int chunk = min(step * WK + wk, p.chunks - 1);  // (behind the last one: the last one again)
+    const int64_t block0 = static_cast<int64_t>(chunk) * p.tiles;
+    const int64_t scale0 = GPC > 1 ? block0 : static_cast<int64_t>(chunk_group(p, chunk)) * p.tiles;
 #pragma unroll
-      for (int c = 0; c < P; ++c)
-        units[buffer * kUnits + ((k * P + c) * MT + (row >> 4)) * 256 + slot * 16 + ((row & 15) ^ slot)] = part[c];
-      // the sums of a group: 16 lanes hold a row's chunk
-      float s = minus24_sum<XT>(x_raw[i]);
-      s = dpp_add<0xb1>(s);
-      s = dpp_add<0x4e>(s);
-      if (GPC <= 2) s = dpp_add<0x141>(s);
-      if (GPC == 1) s = dpp_add<0x140>(s);
-      if (slot % (16 / GPC) == 0) base_lds[buffer][k][slot / (16 / GPC)][row] = s;
+    for (int i = 0; i < NT; ++i) {
+      const int tile = min(tile0 + i, p.tiles - 1);
+      w_raw[slot][i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p.blocks) + (block0 + tile) * 1024 +
+                                                       static_cast<uint32_t>(lane * 16));
+      const int64_t scale_at = (scale0 + tile) * (kTileRows * GPC * SB);
+      s_raw[slot][i] = load_raw_scales<GPC, SB>(static_cast<const char*>(p.scales) + scale_at + static_cast<uint32_t>(n * (GPC * SB)));
+      if (ZEROS)
+        z_raw[slot][i] = load_raw_scales<GPC, SB>(static_cast<const char*>(p.zeros) + scale_at + static_cast<uint32_t>(n * (GPC * SB)));
     }
   };
 
+  const uint32_t unpack_base = base_in_register<XT>();
   f32x4 total[MT][NT];
 #pragma unroll
   for (int a = 0; a < MT; ++a)
 #pragma unroll
     for (int i = 0; i < NT; ++i) total[a][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  const int steps = (p.chunks + WK - 1) / WK;
+  const int steps = ((p.chunks + WK - 1) / WK + kAhead - 1) / kAhead * kAhead;  // (the ones too many count for nothing)
   load_step_x(0);
-  load_step_w(0);
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) load_step_w(k, k);
   store_step_x(0);
   __syncthreads();
-  for (int step = 0; step < steps; ++step) {
-    const int buffer = step & 1;
-    const bool more = step + 1 < steps, there = step * WK + wk < p.chunks;
-    u32x4 w[NT];
-    RawScales<GPC> s[NT], z[NT];
+  for (int step0 = 0; step0 < steps; step0 += kAhead) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) w[i] = w_raw[i], s[i] = s_raw[i], z[i] = z_raw[i];
-    if (more) {
-      load_step_x(step + 1);
-      load_step_w(step + 1);
-    }
-    if (there) {
+    for (int k = 0; k < kAhead; ++k) {
+      const int step = step0 + k, buffer = k & 1;
+      load_step_x(min(step + 1, steps - 1));
+      const uint32_t there = step * WK + wk < p.chunks ? ~0u : 0u;
+      u32x4 b[NT][kSteps];
+      float sc[NT], zero[NT];
+      // 16 rows after the other (a stage each, for every group): operands are read from LDS kReads products ahead, and
+      // while a stage is multiplied the sums of the last one are scaled.
+      constexpr int kStages = GPC * MT, kReads = 2;
+      u32x4 x[kReads + 1][P];
+      constexpr int kBases = (kSteps - 1 + kReads) / kSteps + 1;  // (stages whose operands are being read or multiplied)
+      f32x4 acc[2][NT], base[kBases];
+      auto read_x = [&](int at) {  // operand t of a stage: at = stage * kSteps + t
+        const int stage = at / kSteps, g = stage / MT, a = stage % MT, t = at % kSteps;
+        if (t == 0) base[stage % kBases] = sums_lds[buffer][((wk * MT + a) * GPC + g) * 4 + q];
 #pragma unroll
-      for (int g = 0; g < GPC; ++g) {
-        u32x4 b[NT][kSteps];
-        float sc[NT];
+        for (int c = 0; c < P; ++c)
+          x[at % (kReads + 1)][c] = units[buffer * kUnits + ((wk * MT + a) * P + c) * 256 + (g * kSteps + t) * 64 + lane];
+      };
+      auto scale_rows = [&](int stage) {
+        const int a = stage % MT;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          sc[i] = scale_of<GPC>(s[i], p, g);
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
-          for (int t = 0; t < kSteps; ++t) b[i][t] = unpack<XT>(w[i][g * kSteps + t]);
+          for (int r = 0; r < 4; ++r) total[a][i][r] = fmaf(sc[i], acc[stage & 1][i][r], total[a][i][r]);
+        // (pinned here: left alone, the compiler gathers all of a chunk's scaling behind all of its products, and spills)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(total[a][i]));
+      };
+#pragma unroll
+      for (int at = 0; at < kReads; ++at) read_x(at);
+#pragma unroll
+      for (int stage = 0; stage < kStages; ++stage) {
+        const int g = stage / MT, a = stage % MT;
+        if (a == 0 && g > 0) scale_rows(stage - 1);  // (before the group's scales are replaced)
+        if (a == 0) {
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            sc[i] = scale_of<GPC, SB>(s_raw[k][i], p, g, there);
+            if (ZEROS) zero[i] = scale_of<GPC, SB>(z_raw[k][i], p, g, there) * (-1.0f / 24.0f);
+          }
         }
 #pragma unroll
-        for (int a = 0; a < MT; ++a) {
-          const f32x4 base = *reinterpret_cast<const f32x4*>(&base_lds[buffer][wk][g][16 * a + 4 * q]);
-          f32x4 acc[NT];
+        for (int t = 0; t < kSteps; ++t) {
+          const int at = stage * kSteps + t;
+          if (at + kReads < kStages * kSteps) read_x(at + kReads);
 #pragma unroll
-          for (int i = 0; i < NT; ++i) acc[i] = base;
+          for (int i = 0; i < NT; ++i) {
+            if (a == 0) b[i][t] = unpack<XT>(w_raw[k][i][g * kSteps + t], unpack_base);
 #pragma unroll
-          for (int t = 0; t < kSteps; ++t) {
-            const int slot = 4 * (g * kSteps + t) + q;
-#pragma unroll
-            for (int c = 0; c < P; ++c) {
-              const u32x4 x = units[buffer * kUnits + ((wk * P + c) * MT + a) * 256 + slot * 16 + (n ^ slot)];
-#pragma unroll
-              for (int i = 0; i < NT; ++i) acc[i] = M::product(x, b[i][t], acc[i]);
-            }
+            for (int c = 0; c < P; ++c)
+              acc[stage & 1][i] = M::product(x[at % (kReads + 1)][c], b[i][t], t == 0 && c == 0 ? base[stage % kBases] : acc[stage & 1][i]);
           }
+        }
+        if (ZEROS) {
 #pragma unroll
           for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) total[a][i][r] = fmaf(sc[i], acc[i][r], total[a][i][r]);
-          if (p.zeros) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-              const float zero = scale_of<GPC>(z[i], p, g) * (-1.0f / 24.0f);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) total[a][i][r] = fmaf(zero, base[r], total[a][i][r]);
-            }
-          }
+            for (int r = 0; r < 4; ++r) total[a][i][r] = fmaf(zero[i], base[stage % kBases][r], total[a][i][r]);
         }
+        if (a == 0 && g == GPC - 1) load_step_w(step + kAhead, k);
+        if (a > 0) scale_rows(stage - 1);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      scale_rows(kStages - 1);
+      __builtin_amdgcn_sched_barrier(0);
+      store_step_x(buffer ^ 1);
+      __syncthreads();
     }
-    if (more) store_step_x(buffer ^ 1);
-    __syncthreads();
   }
 
   // 16 rows at a time through LDS: a lane then has 16 / (4 / NT) .. consecutive entries of a row to store

@@ -27,8 +27,8 @@ extern "C" {
 typedef struct ets_logit_head ets_logit_head;
 
 /* Lays the weights out for the kernels in memory of its own on the current HIP device (as large as the
- * packed weights, rounded up to 16 rows x 128 columns, plus the scales) and waits for `hip_stream`, so
- * the caller may free its own copy when the call returns.  All pointers are DEVICE pointers:
+ * packed weights, rounded up to 16 rows x 128 columns, plus the scales; and a work buffer of about 1 KiB
+ * per hidden column) and waits for `hip_stream`, so the caller may free its own copy when the call returns.  All pointers are DEVICE pointers:
  *   d_packed  uint8 [vocab, (hidden + 1) / 2], rows `packed_stride` bytes apart
  *   d_scales  [vocab, ceil(hidden / group)] of `scale_dtype` (Float, Half or BFloat16), contiguous
  *   d_zeros   the same shape and type, or NULL for symmetric weights
@@ -41,8 +41,9 @@ ETS_API ets_status ets_logit_head_destroy(ets_logit_head* h);
 
 /* Logits of `rows` hidden states, asynchronously on `hip_stream`; allocates nothing, may be captured.
  * d_hidden: [rows, hidden] of `dtype`, d_logits: [rows, vocab] of `logits_dtype` (each Float, Half or
- * BFloat16), rows the given numbers of elements apart (innermost stride 1).  Calls on one handle only
- * read it, so they may overlap on several streams. */
+ * BFloat16), rows the given numbers of elements apart (innermost stride 1).  Calls with more than 16 rows
+ * share a work buffer of the handle: issue them, and the graphs that captured them, on one stream at a
+ * time.  Calls with at most 16 rows only read the handle and may overlap with any others. */
 ETS_API ets_status ets_logit_head_logits(ets_logit_head* h, const void* d_hidden, int32_t dtype, int32_t rows,
                                          int64_t hidden_stride, void* d_logits, int32_t logits_dtype, int64_t logits_stride,
                                          void* hip_stream);
