@@ -396,7 +396,7 @@ head_tile_kernel(const HeadParams p) {
   constexpr int kCopies = kUnits / kLanes;   // of them per lane
   constexpr int kSums = WK * MT * GPC * 4;   // quadruples of row sums per step
   static_assert(kUnits % kLanes == 0 && kSums <= kLanes, "");
-  constexpr int kOut = WK * WV * 16 * NT * 16;  // floats of 16 rows of the result
+  constexpr int kOut = WK * WV * 16 * NT * 16;  // floats of 16 rows of the result, per wave
   constexpr int kBytes = 2 * kUnits * 16 > kOut * 4 ? 2 * kUnits * 16 : kOut * 4;
   __shared__ __attribute__((aligned(16))) char lds[kBytes];
   __shared__ f32x4 sums_lds[2][kSums];
@@ -411,14 +411,11 @@ head_tile_kernel(const HeadParams p) {
   const int m0 = row_block * kRows, tile0 = (vocab_block * WV + wv) * NT;
   const int row_tiles = (p.rows + 15) / 16;
 
-  // Weights and scales run kAhead steps ahead, hidden states one: their loads are issued first in a step, so that waiting
-  // for them does not wait for the weights behind them.  Each slot of the ring has registers of its own (the loop is
-  // unrolled kAhead times): a copy would wait for what is copied.
-  constexpr int kAhead = 2;
-  static_assert(kAhead % 2 == 0 && kChunkRound % (kAhead * WK) == 0, "the buffers in LDS alternate with the slots; whole rounds");
-  u32x4 x_raw[kCopies], w_raw[kAhead][NT];
+  // The next step's hidden states are loaded first, so that waiting for them does not wait for the weights behind them.
+  static_assert(kChunkRound % (2 * WK) == 0, "whole rounds of two steps");
+  u32x4 x_raw[kCopies], w_raw[NT];
   f32x4 sums_raw;
-  RawScales<GPC, SB> s_raw[kAhead][NT], z_raw[kAhead][NT];
+  RawScales<GPC, SB> s_raw[NT], z_raw[NT];
   // Unit u of a step: chunk u / (256 P MT) of it, 16-row tile u / (256 P) % MT (of those that do not exist the last one).
   // Everything but the lane's offset is the same in every lane of a wave.
   const int work_chunks = padded_chunks(p.chunks);
@@ -440,19 +437,19 @@ head_tile_kernel(const HeadParams p) {
     sums_lds[buffer][sum_u] = sums_raw;
   };
   // (all of these offsets but the lane's are the same in every lane)
-  auto load_step_w = [&](int step, int slot) {
+  auto load_step_w = [&](int step) {
     const int chunk = min(step * WK + wk, p.chunks - 1);  // (behind the last one: the last one again)
     const int64_t block0 = static_cast<int64_t>(chunk) * p.tiles;
     const int64_t scale0 = GPC > 1 ? block0 : static_cast<int64_t>(chunk_group(p, chunk)) * p.tiles;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int tile = min(tile0 + i, p.tiles - 1);
-      w_raw[slot][i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p.blocks) + (block0 + tile) * 1024 +
+      w_raw[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p.blocks) + (block0 + tile) * 1024 +
                                                        static_cast<uint32_t>(lane * 16));
       const int64_t scale_at = (scale0 + tile) * (kTileRows * GPC * SB);
-      s_raw[slot][i] = load_raw_scales<GPC, SB>(static_cast<const char*>(p.scales) + scale_at + static_cast<uint32_t>(n * (GPC * SB)));
+      s_raw[i] = load_raw_scales<GPC, SB>(static_cast<const char*>(p.scales) + scale_at + static_cast<uint32_t>(n * (GPC * SB)));
       if (ZEROS)
-        z_raw[slot][i] = load_raw_scales<GPC, SB>(static_cast<const char*>(p.zeros) + scale_at + static_cast<uint32_t>(n * (GPC * SB)));
+        z_raw[i] = load_raw_scales<GPC, SB>(static_cast<const char*>(p.zeros) + scale_at + static_cast<uint32_t>(n * (GPC * SB)));
     }
   };
 
@@ -463,16 +460,15 @@ head_tile_kernel(const HeadParams p) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) total[a][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  const int steps = ((p.chunks + WK - 1) / WK + kAhead - 1) / kAhead * kAhead;  // (the ones too many count for nothing)
+  const int steps = ((p.chunks + WK - 1) / WK + 1) / 2 * 2;  // (the one too many counts for nothing)
   load_step_x(0);
-#pragma unroll
-  for (int k = 0; k < kAhead; ++k) load_step_w(k, k);
+  load_step_w(0);
   store_step_x(0);
   __syncthreads();
-  for (int step0 = 0; step0 < steps; step0 += kAhead) {
+  for (int step0 = 0; step0 < steps; step0 += 2) {
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int step = step0 + k, buffer = k & 1;
+    for (int buffer = 0; buffer < 2; ++buffer) {
+      const int step = step0 + buffer;
       load_step_x(min(step + 1, steps - 1));
       const uint32_t there = step * WK + wk < p.chunks ? ~0u : 0u;
       u32x4 b[NT][kSteps];
@@ -509,8 +505,8 @@ head_tile_kernel(const HeadParams p) {
         if (a == 0) {
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
-            sc[i] = scale_of<GPC, SB>(s_raw[k][i], p, g, there);
-            if (ZEROS) zero[i] = scale_of<GPC, SB>(z_raw[k][i], p, g, there) * (-1.0f / 24.0f);
+            sc[i] = scale_of<GPC, SB>(s_raw[i], p, g, there);
+            if (ZEROS) zero[i] = scale_of<GPC, SB>(z_raw[i], p, g, there) * (-1.0f / 24.0f);
           }
         }
 #pragma unroll
@@ -519,7 +515,7 @@ head_tile_kernel(const HeadParams p) {
           if (at + kReads < kStages * kSteps) read_x(at + kReads);
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
-            if (a == 0) b[i][t] = unpack<XT>(w_raw[k][i][g * kSteps + t], unpack_base);
+            if (a == 0) b[i][t] = unpack<XT>(w_raw[i][g * kSteps + t], unpack_base);
 #pragma unroll
             for (int c = 0; c < P; ++c)
               acc[stage & 1][i] = M::product(x[at % (kReads + 1)][c], b[i][t], t == 0 && c == 0 ? base[stage % kBases] : acc[stage & 1][i]);
@@ -531,7 +527,7 @@ head_tile_kernel(const HeadParams p) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) total[a][i][r] = fmaf(zero[i], base[stage % kBases][r], total[a][i][r]);
         }
-        if (a == 0 && g == GPC - 1) load_step_w(step + kAhead, k);
+        if (a == 0 && g == GPC - 1) load_step_w(step + 1);
         if (a > 0) scale_rows(stage - 1);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -542,26 +538,43 @@ head_tile_kernel(const HeadParams p) {
     }
   }
 
-  // 16 rows at a time through LDS: a lane then has 16 / (4 / NT) .. consecutive entries of a row to store
+  // 16 rows at a time through LDS; a lane then stores 16 (NT = 4) or 8 consecutive entries of a row.  With WK = 1 a wave has a
+  // place of its own there and waits for nobody.
+  constexpr int kMine = 16 * NT * 16;  // floats of a wave
   float* result = reinterpret_cast<float*>(lds);
-  constexpr int kWide = NT * 16 * WV;  // vocabulary entries of the workgroup
+  float* mine = result + wave * kMine;
+  constexpr int kRun = NT * 4;
+  const int row = lane >> 2, col = (lane & 3) * kRun;
 #pragma unroll
   for (int a = 0; a < MT; ++a) {
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) result[(wk * 16 + 4 * q + r) * kWide + (wv * NT + i) * 16 + n] = total[a][i][r];
-    __syncthreads();
-    for (int e = tid * 4; e < 16 * kWide; e += kLanes * 4) {
-      const int row = e / kWide, col = e % kWide, m = m0 + 16 * a + row, v = vocab_block * kWide + col;
-      if (m < p.rows) {
-        f32x4 y = *reinterpret_cast<const f32x4*>(&result[row * kWide + col]);
+      for (int r = 0; r < 4; ++r) mine[(4 * q + r) * (NT * 16) + i * 16 + n] = total[a][i][r];
+    if (WK > 1) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    const int m = m0 + 16 * a + row, v = tile0 * 16 + col;
+    if (wk == 0 && m < p.rows) {
 #pragma unroll
-        for (int k = 1; k < WK; ++k) y += *reinterpret_cast<const f32x4*>(&result[(k * 16 + row) * kWide + col]);
-        store_logits(p, m, v, y);
+      for (int j = 0; j < kRun; j += 4) {
+        f32x4 y = *reinterpret_cast<const f32x4*>(&mine[row * (NT * 16) + col + j]);
+#pragma unroll
+        for (int k = 1; k < WK; ++k) y += *reinterpret_cast<const f32x4*>(&mine[k * WV * kMine + row * (NT * 16) + col + j]);
+        store_logits(p, m, v + j, y);
       }
     }
-    __syncthreads();
+    if (WK > 1) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
   }
 }
 
