@@ -24,6 +24,7 @@ namespace ets {
 constexpr int kHeadBlock = 256;  // lanes of a workgroup
 constexpr int kTileRows = 16;    // vocabulary rows of a block
 constexpr int kChunkCols = 128;  // columns of a block
+constexpr int kRowsBeside = 5;   // rows of fp32 whose three parts fit one operand of 16 rows
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -220,18 +221,45 @@ __device__ __forceinline__ void store_logits(const HeadParams& p, int m, int v, 
 }
 
 // ---- the product, few rows --------------------------------------------------------------------------------
+// One of the three parts of fp32 columns, as operand A: `first` is 0xffff0000 for all but the highest part, `second`
+// for the lowest, otherwise 0.
+__device__ __forceinline__ u32x4 part_of_x(const RawX<kDtypeFloat>& x, uint32_t first, uint32_t second) {
+  u32x4 part;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t bits = x.v[i >> 1][2 * (i & 1) + h];
+      const float rest = __uint_as_float(bits) - __uint_as_float(bits & first);
+      v[h] = __float_as_uint(rest - __uint_as_float(__float_as_uint(rest) & second));
+    }
+    part[i] = (v[0] >> 16) | (v[1] & 0xffff0000u);
+  }
+  return part;
+}
+
 // A workgroup makes 16 rows x (16 NT) vocabulary entries; its four waves take the chunks of columns in turn
-// and their sums are added up in a fixed order at the end.
-template <int XT, int GPC, int SB, bool ZEROS, int NT>
+// and their sums are added up in a fixed order at the end.  BESIDE, for up to five rows of fp32: the parts of a row
+// are three rows of the same operand, 5 apart, instead of three operands.
+//
+// Bound by the reads of the weights: 128256 x 4096 in groups of 128, 272 MB, in 49 us, 5.5 TB/s, where a kernel that
+// only reads reaches 5.95 TB/s.  x comes from the caches for every NT tiles again, which is what holds back fp32 (50257 x
+// 1601, 3 rows: 3.1 TB/s; 20 us with an operand for each part).  No copy of the next chunk's weights in a second set
+// of registers: it halves the waves on a SIMD and is slower everywhere (128256 x 4096: 51 us; 151936 x 5120 with
+// zeros: 105 us instead of 93).
+template <int XT, int GPC, int SB, bool ZEROS, int NT, bool BESIDE>
 __global__ void __launch_bounds__(kHeadBlock)
 head_stream_kernel(const HeadParams p) {
   using M = Matrix<XT>;
-  constexpr int P = Parts<XT>::value, kWavesHere = kHeadBlock / 64, kSteps = 4 / GPC;  // products per group of a chunk
+  constexpr int P = BESIDE ? 1 : Parts<XT>::value, kWavesHere = kHeadBlock / 64, kSteps = 4 / GPC;  // products per group of a chunk
   __shared__ float red[kWavesHere][NT][64 * 4];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, q = lane >> 4;
   const int tile0 = blockIdx.x * NT, m0 = blockIdx.y * 16;
-  const bool exists = m0 + n < p.rows;
-  const char* x_row = static_cast<const char*>(p.x) + (exists ? m0 + n : 0) * p.x_stride * ElemSize<XT>::value;
+  const int part = BESIDE ? n / kRowsBeside : 0, row = m0 + (BESIDE ? n % kRowsBeside : n);
+  const bool exists = row < p.rows && part < 3;
+  const uint32_t first = part >= 1 ? 0xffff0000u : 0u, second = part >= 2 ? 0xffff0000u : 0u;
+  const char* x_row = static_cast<const char*>(p.x) + (exists ? row : 0) * p.x_stride * ElemSize<XT>::value;
   const u32x4 minus24 = {M::kMinus24, M::kMinus24, M::kMinus24, M::kMinus24}, one = {M::kOne, M::kOne, M::kOne, M::kOne};
   const uint32_t unpack_base = base_in_register<XT>();
   f32x4 total[NT];
@@ -250,7 +278,14 @@ head_stream_kernel(const HeadParams p) {
     }
     u32x4 x[4][P];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) split_x<XT>(load_raw_x<XT>(x_row, chunk * kChunkCols + 32 * t + 8 * q, p.hidden, exists), x[t]);
+    for (int t = 0; t < 4; ++t) {
+      const RawX<XT> raw = load_raw_x<XT>(x_row, chunk * kChunkCols + 32 * t + 8 * q, p.hidden, exists);
+      if constexpr (BESIDE) {
+        x[t][0] = part_of_x(raw, first, second);
+      } else {
+        split_x<XT>(raw, x[t]);
+      }
+    }
 #pragma unroll
     for (int g = 0; g < GPC; ++g) {
       f32x4 base = {0.0f, 0.0f, 0.0f, 0.0f}, sums = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -283,14 +318,18 @@ head_stream_kernel(const HeadParams p) {
   for (int i = 0; i < NT; ++i) *reinterpret_cast<f32x4*>(&red[wave][i][lane * 4]) = total[i];
   __syncthreads();
   // row m of the tile is element m & 3 of the lanes 16 (m >> 2) + column
-  for (int e = tid; e < NT * 256; e += kHeadBlock) {
+  const int rows_here = min(BESIDE ? kRowsBeside : 16, p.rows - m0);
+  for (int e = tid; e < NT * 16 * rows_here; e += kHeadBlock) {
     const int col = e & (16 * NT - 1), m = e / (16 * NT);
-    const int at = ((m >> 2) * 16 + (col & 15)) * 4 + (m & 3);
-    float y = red[0][col >> 4][at];
+    float y = 0.0f;
 #pragma unroll
-    for (int k = 1; k < kWavesHere; ++k) y += red[k][col >> 4][at];
+    for (int i = BESIDE ? 2 : 0; i >= 0; --i) {
+      const int at_m = m + i * kRowsBeside, at = ((at_m >> 2) * 16 + (col & 15)) * 4 + (at_m & 3);
+#pragma unroll
+      for (int k = 0; k < kWavesHere; ++k) y += red[k][col >> 4][at];
+    }
     const int v = tile0 * kTileRows + col;
-    if (m0 + m < p.rows && v < p.vocab) store_logit(p, m0 + m, v, y);
+    if (v < p.vocab) store_logit(p, m0 + m, v, y);
   }
 }
 

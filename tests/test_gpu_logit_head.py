@@ -97,6 +97,29 @@ def test_wide_values(dev):
     check(head.logits(eye), eye, w, group, "f32", "columns")
 
 
+@pytest.mark.parametrize("rows", [1, 3, 5, 6, 16, 21])
+def test_wide_values_in_few_rows(dev, rows):
+    """Up to five rows of fp32 have their parts beside each other in one operand, more have an operand for each."""
+    vocab, hidden, group = 80, 500, 32
+    w = weights(22, vocab, hidden, group, "f32", True, dev)
+    head = ea.LogitHead(w[0], w[1], group, zeros=w[2])
+    g = np.random.default_rng(rows)
+    x = torch.from_numpy((g.standard_normal((rows, hidden)) * 2.0 ** g.integers(-60, 60, size=(rows, hidden))).astype(np.float32)).to(dev)
+    check(head.logits(x), x, w, group, "f32", rows)
+    for first in range(0, hidden - rows, 97):
+        eye = torch.eye(hidden, device=dev)[first:first + rows] * 1.2345678
+        check(head.logits(eye), eye, w, group, "f32", (rows, first))
+
+
+@pytest.mark.parametrize("dtype,rows,group,zeros", [("f16", 5, 64, True), ("bf16", 16, 32, False), ("f32", 2, 128, True), ("f32", 7, 32, False)])
+def test_long_vocabularies(dev, dtype, rows, group, zeros):
+    vocab, hidden = 70001, 260  # more than 4096 tiles of 16
+    w = weights(12, vocab, hidden, group, "f32", zeros, dev)
+    x = states(4, rows, hidden, dtype, dev)
+    head = ea.LogitHead(w[0], w[1], group, hidden_size=hidden, zeros=w[2])
+    check(head.logits(x, dtype=torch.float32), x, w, group, "f32", (dtype, rows, group))
+
+
 @pytest.mark.parametrize("rows", [1, 20, 100])
 def test_strides_gaps_and_what_lies_beside(dev, rows):
     vocab, hidden, group = 203, 301, 64
