@@ -48,6 +48,10 @@ hipError_t launch_verify(ets::VerifyParams p, int num_cus, hipStream_t stream) {
   p.step_j = static_cast<int32_t>(stride / p.chunks % p.rows_per_seq);
   p.step_b = static_cast<int32_t>(stride / p.chunks / p.rows_per_seq);
   hipLaunchKernelGGL((ets::verify_stats_kernel<DT>), dim3(static_cast<uint32_t>(groups)), dim3(ets::kVerifyBlock), 0, stream, p);
+  if (!p.temperatures && p.temperature == 0.0f) {
+    hipLaunchKernelGGL((ets::verify_greedy_kernel<DT>), dim3(p.sequences), dim3(ets::kVerifyBlock), 0, stream, p);
+    return hipGetLastError();
+  }
   // With up to two workgroups per CU in verify_rest the decision costs less inside it than a launch would.
   const int64_t chunks = static_cast<int64_t>(p.sequences) * p.chunks;
   if (chunks > 2 * num_cus) {
@@ -153,7 +157,8 @@ ets_status ets_verifier_verify(ets_verifier* v, const ets_verify_batch* a, void*
     return verifier_fail(v, ETS_INVALID_ARGUMENT, "ets_verifier_verify: pointer not aligned to its element type");
   ets::VerifyParams p = {};
   p.target = a->target_logits;
-  p.draft = with_draft ? a->draft_logits : nullptr;
+  const bool all_greedy = !a->temperatures && a->temperature == 0.0f;  // (nothing of the draft model is read)
+  p.draft = with_draft && !all_greedy ? a->draft_logits : nullptr;
   p.target_seq = a->target_sequence_stride;
   p.target_pos = a->target_position_stride;
   p.draft_seq = a->draft_sequence_stride;

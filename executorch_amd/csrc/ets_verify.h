@@ -544,6 +544,28 @@ verify_decide_kernel(const VerifyParams p) {
   if (threadIdx.x == 0) p.decisions[blockIdx.x] = dec;
 }
 
+// Writes a sequence's tokens and their number: by every lane, `own` being its draft (read before: the tokens may
+// go where the drafts are).  kMaxDrafts is below the workgroup's size.
+__device__ __forceinline__ void write_answer(const VerifyParams& p, int b, int kept, int own, int token) {
+  const int tid = threadIdx.x;
+  if (tid <= p.drafts) p.tokens[b * p.tokens_stride + tid] = tid < kept ? own : (tid == kept ? token : -1);
+  if (tid == 0) p.accepted[b] = kept;
+}
+__device__ __forceinline__ int own_draft(const VerifyParams& p, int b) {
+  return threadIdx.x < p.drafts ? p.draft_tokens[b * p.draft_tokens_stride + threadIdx.x] : -1;
+}
+
+// All there is to do behind the statistics if every sequence is greedy: one launch instead of three (64 x 4 at
+// 128256 bf16: 22 us against 26; 1 x 4: 7 against 9).
+template <int DT>
+__global__ void __launch_bounds__(kVerifyBlock)
+verify_greedy_kernel(const VerifyParams p) {
+  __shared__ DecideSpace lds;
+  const int own = own_draft(p, blockIdx.x);
+  const Decision dec = decide<DT>(p, blockIdx.x, lds);
+  write_answer(p, blockIdx.x, dec.kept, own, dec.answer);
+}
+
 // ---- mass of every chunk ------------------------------------------------------------------------
 // The residual max(a / Zt - b / Zd, 0) = max(a - rho b, 0) / Zt needs the rows' exact sums before its own can be
 // taken.  One pass does for both: with the statistics' rho, usually off by some 1e-7, and B the sum of b over
@@ -629,15 +651,14 @@ verify_finish_kernel(const VerifyParams p) {
   ChunkMass* mass = p.mass + static_cast<int64_t>(b) * p.chunks;
   ChunkMass mass0 = {};  // of chunk `lane`: on its way while the decision is read
   if (wave == 0 && lane < p.chunks) mass0 = mass[lane];
-  const int own = tid < p.drafts ? p.draft_tokens[b * p.draft_tokens_stride + tid] : -1;  // (before the answer is written: it may go to the same place)
+  const int own = own_draft(p, b);
   const float coin = p.coins[b * p.coins_stride + p.drafts];
   const Decision dec = p.decisions[b];
-  int32_t* out = p.tokens + b * p.tokens_stride;
-  auto answer = [&](int token) {  // (by every lane, with the same token; kMaxDrafts is below the workgroup's size)
-    if (tid <= p.drafts) out[tid] = tid < dec.kept ? own : (tid == dec.kept ? token : -1);
-    if (tid == 0) p.accepted[b] = dec.kept;
-  };
-  if (dec.draw == kDrawNone) return answer(dec.answer);
+  auto answer = [&](int token) { write_answer(p, b, dec.kept, own, token); };
+  if (dec.draw == kDrawNone) {
+    __syncthreads();  // (with 64 drafts the answer's last token is written by another wave than reads the drafts)
+    return answer(dec.answer);
+  }
 
   const RowWeights t_weight(dec.t_max, dec.temperature), d_weight(dec.d_max, dec.temperature);
   auto chunk_mass = [&](int k) { return k < 64 ? mass0 : mass[k]; };

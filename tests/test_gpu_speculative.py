@@ -142,6 +142,25 @@ def test_masked_rows_and_rows_without_a_distribution(dev, dtype, draft):
     check(ea.DraftVerifier(V, S, K), x, (dtype, draft, "greedy"))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("S,K,V", [(1, 0, 5), (1, 4, 32000), (9, 3, 2049), (70, 2, 700), (2, 64, 4100)])
+def test_one_temperature_of_zero(dev, dtype, S, K, V):
+    """A number for all sequences takes fewer launches than their own temperatures do; in place, drafts shifted by one."""
+    x = problem(S + K, S, K, V, dtype, dev, ragged=K > 0, temps=(0.0,))
+    x["target"][S // 2, 0, V - 1] = float("nan")
+    x["target"][S - 1, K, :] = -float("inf")
+    t, a = want(x)
+    v = ea.DraftVerifier(V, S, K)
+    check(v, x, "own temperatures")
+    for place in (slice(0, K), slice(1, K + 1)):
+        for temperature in (0.0, x["temperature"]):
+            both = torch.full((S, K + 1), 7, dtype=torch.int32, device=dev)
+            both[:, place] = x["tokens"]
+            tokens, accepted = v.verify(x["target"], both[:, place], x["coins"], draft_logits=x["draft"], draft_lengths=x["lengths"],
+                                        temperature=temperature, tokens_out=both)
+            assert np.array_equal(accepted.cpu().numpy(), a) and np.array_equal(tokens.cpu().numpy(), t)
+
+
 def test_odd_coins_and_temperatures(dev):
     S, K, V = 10, 3, 5003
     x = problem(17, S, K, V, "f32", dev)
