@@ -49,13 +49,13 @@ hipError_t launch_verify(ets::VerifyParams p, int num_cus, hipStream_t stream) {
   p.step_b = static_cast<int32_t>(stride / p.chunks / p.rows_per_seq);
   hipLaunchKernelGGL((ets::verify_stats_kernel<DT>), dim3(static_cast<uint32_t>(groups)), dim3(ets::kVerifyBlock), 0, stream, p);
   if (!p.temperatures && p.temperature == 0.0f) {
-    hipLaunchKernelGGL((ets::verify_greedy_kernel<DT>), dim3(p.sequences), dim3(ets::kVerifyBlock), 0, stream, p);
+    hipLaunchKernelGGL((ets::verify_greedy_kernel<DT>), dim3(p.sequences), dim3(64 * ets::kDecideWaves), 0, stream, p);
     return hipGetLastError();
   }
   // With up to two workgroups per CU in verify_rest the decision costs less inside it than a launch would.
   const int64_t chunks = static_cast<int64_t>(p.sequences) * p.chunks;
   if (chunks > 2 * num_cus) {
-    hipLaunchKernelGGL((ets::verify_decide_kernel<DT>), dim3(p.sequences), dim3(ets::kVerifyBlock), 0, stream, p);
+    hipLaunchKernelGGL((ets::verify_decide_kernel<DT>), dim3(p.sequences), dim3(64 * ets::kDecideWaves), 0, stream, p);
     hipLaunchKernelGGL((ets::verify_rest_kernel<DT, true>), dim3(static_cast<uint32_t>(chunks)), dim3(ets::kVerifyBlock), 0, stream, p);
   } else {
     hipLaunchKernelGGL((ets::verify_rest_kernel<DT, false>), dim3(static_cast<uint32_t>(chunks)), dim3(ets::kVerifyBlock), 0, stream, p);

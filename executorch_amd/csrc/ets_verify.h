@@ -396,29 +396,32 @@ __device__ __forceinline__ void combine_chunks(const ChunkStat* const* st, int c
   }
 }
 
+// Waves of a workgroup that only decides, a row each at a time (64 x 4 at 128256 with 4 waves of three rows: 5.9 us,
+// with 16: 4.8; 33 x 7 at 151936: 10.6 and 5.5).
+constexpr int kDecideWaves = 16;
 struct DecideSpace {  // in LDS
   RowNorm rows[2 * kMaxDrafts + 1];
   double table[kExp2Steps];
-  double red[kVerifyWaves];
+  double red[kDecideWaves];
   uint64_t near;  // drafts whose coin is too close to tell
   uint64_t accept, valid;
 };
 
 // The row's sum in 64 bits, by the whole workgroup.
-template <int DT>
+template <int DT, int WAVES>
 __device__ __forceinline__ double exact_sum(const VerifyParams& p, const char* row, float max, float temperature, DecideSpace& lds) {
   const RowWeights weight(max, temperature);
   double sum = 0.0;
 #pragma unroll 1
-  for (int i = threadIdx.x; i < p.vocab; i += kVerifyBlock) sum += weight(load_elem<DT>(row, i), lds.table);
-  return block_sum_f64<kVerifyWaves>(sum, lds.red);
+  for (int i = threadIdx.x; i < p.vocab; i += 64 * WAVES) sum += weight(load_elem<DT>(row, i), lds.table);
+  return block_sum_f64<WAVES>(sum, lds.red);
 }
 
 // What happens to a sequence, worked out by a workgroup from the statistics (in small batches every
 // workgroup of verify_rest does so for itself: it is a few hundred bytes and two exponentials per draft).
-template <int DT>
+template <int DT, int WAVES>
 __device__ __forceinline__ Decision decide(const VerifyParams& p, int b, DecideSpace& lds) {
-  constexpr int R = 3;
+  constexpr int R = WAVES == kDecideWaves ? 1 : 3;  // rows a wave takes at once
   const int tid = threadIdx.x, wave = tid >> 6;
   Decision out;
   const int len = sequence_length(p, b);
@@ -442,7 +445,7 @@ __device__ __forceinline__ Decision decide(const VerifyParams& p, int b, DecideS
   const bool inside = x >= 0 && x < p.vocab;
   // the sequence's rows: target 0 .. len, and draft 0 .. len - 1 unless it is greedy
   const int count = len + 1 + (p.draft && !greedy ? len : 0);
-  for (int k = wave * R; k < count; k += kVerifyWaves * R) {
+  for (int k = wave * R; k < count; k += WAVES * R) {
     const ChunkStat* src[R];
     RowNorm norm[R];
     int at[R];
@@ -497,8 +500,8 @@ __device__ __forceinline__ Decision decide(const VerifyParams& p, int b, DecideS
     if (i > first_stop()) break;
     nears &= nears - 1;
     const RowNorm t = lds.rows[i], d = p.draft ? lds.rows[p.drafts + 1 + i] : RowNorm{1.0, 0.0f, 0};
-    const double t_sum = exact_sum<DT>(p, target_row<DT>(p, b, i), t.max, temperature, lds);
-    const double d_sum = p.draft ? exact_sum<DT>(p, draft_row<DT>(p, b, i), d.max, temperature, lds) : 1.0;
+    const double t_sum = exact_sum<DT, WAVES>(p, target_row<DT>(p, b, i), t.max, temperature, lds);
+    const double d_sum = p.draft ? exact_sum<DT, WAVES>(p, draft_row<DT>(p, b, i), d.max, temperature, lds) : 1.0;
     if (tid == i) {
       const double q = p.draft ? exact_weight(d_logit, d.max, temperature) / d_sum : 1.0;
       const bool accept = static_cast<double>(coin) * q < exact_weight(t_logit, t.max, temperature) / t_sum;
@@ -537,10 +540,10 @@ __device__ __forceinline__ Decision decide(const VerifyParams& p, int b, DecideS
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kVerifyBlock)
+__global__ void __launch_bounds__(64 * kDecideWaves)
 verify_decide_kernel(const VerifyParams p) {
   __shared__ DecideSpace lds;
-  const Decision dec = decide<DT>(p, blockIdx.x, lds);
+  const Decision dec = decide<DT, kDecideWaves>(p, blockIdx.x, lds);
   if (threadIdx.x == 0) p.decisions[blockIdx.x] = dec;
 }
 
@@ -558,11 +561,11 @@ __device__ __forceinline__ int own_draft(const VerifyParams& p, int b) {
 // All there is to do behind the statistics if every sequence is greedy: one launch instead of three (64 x 4 at
 // 128256 bf16: 22 us against 26; 1 x 4: 7 against 9).
 template <int DT>
-__global__ void __launch_bounds__(kVerifyBlock)
+__global__ void __launch_bounds__(64 * kDecideWaves)
 verify_greedy_kernel(const VerifyParams p) {
   __shared__ DecideSpace lds;
   const int own = own_draft(p, blockIdx.x);
-  const Decision dec = decide<DT>(p, blockIdx.x, lds);
+  const Decision dec = decide<DT, kDecideWaves>(p, blockIdx.x, lds);
   write_answer(p, blockIdx.x, dec.kept, own, dec.answer);
 }
 
@@ -585,7 +588,7 @@ verify_rest_kernel(const VerifyParams p) {
     dec = p.decisions[b];
     if (tid < kExp2Steps) lds.table[tid] = p.exp2_table[tid];
   } else {
-    dec = decide<DT>(p, b, lds);
+    dec = decide<DT, kVerifyWaves>(p, b, lds);
     if (chunk == 0 && tid == 0) p.decisions[b] = dec;
   }
   if (dec.draw == kDrawNone) return;  // (the same in every lane)
