@@ -35,7 +35,7 @@ class LogitHead:
         for t, name in ((scales, "scales"), (zeros, "zeros")):
             if t is not None and not (t.device == packed.device and t.shape == shape and t.is_contiguous() and t.dtype == scales.dtype):
                 raise SamplerError(_capi.INVALID_ARGUMENT, f"{name} must be a contiguous tensor {list(shape)} next to packed, scales and zeros of one type")
-        self.device = packed.device
+        self.device, self._index = packed.device, packed.get_device()
         with torch.cuda.device(self.device):
             st = _capi.lib().ets_logit_head_create(
                 vocab, hidden, group_size, packed.data_ptr(), packed.stride(0), scales.data_ptr(),
@@ -43,6 +43,7 @@ class LogitHead:
                 torch.cuda.current_stream(self.device).cuda_stream, C.byref(self._h))
         if st != _capi.OK:
             raise SamplerError(st, _capi.lib().ets_logit_head_last_error(None).decode())
+        self._logits = _capi.lib().ets_logit_head_logits
         self.vocab_size, self.hidden_size, self.group_size = vocab, hidden, group_size
 
     def close(self) -> None:
@@ -60,20 +61,19 @@ class LogitHead:
         """``hidden`` ``[rows, hidden]`` (fp32, fp16 or bf16, unit inner stride) -> ``[rows, vocab]`` of ``dtype``
         (default: that of ``out``, or of ``hidden``), asynchronously on the current stream."""
         out = self._output(hidden, out, dtype)
-        st = _capi.lib().ets_logit_head_logits(self._h, hidden.data_ptr(), dtype_code(hidden), hidden.shape[0], hidden.stride(0),
-                                               out.data_ptr(), dtype_code(out), out.stride(0),
-                                               torch.cuda.current_stream(self.device).cuda_stream)
+        st = self._logits(self._h, hidden.data_ptr(), dtype_code(hidden), hidden.shape[0], hidden.stride(0), out.data_ptr(),
+                          dtype_code(out), out.stride(0), torch._C._cuda_getCurrentRawStream(self._index))
         if st != _capi.OK:
             raise SamplerError(st, _capi.lib().ets_logit_head_last_error(self._h).decode())
         return out
 
     def _output(self, hidden, out, dtype) -> torch.Tensor:
-        if hidden.device != self.device or hidden.dim() != 2 or hidden.shape[1] != self.hidden_size or \
+        if hidden.get_device() != self._index or hidden.dim() != 2 or hidden.shape[1] != self.hidden_size or \
                 (hidden.stride(1) != 1 and self.hidden_size > 1):
             raise SamplerError(_capi.INVALID_ARGUMENT, f"hidden must be [rows, {self.hidden_size}] on {self.device} with unit inner stride")
         if out is None:
             return torch.empty((hidden.shape[0], self.vocab_size), dtype=dtype or hidden.dtype, device=self.device)
-        if out.device != self.device or out.shape != (hidden.shape[0], self.vocab_size) or (out.stride(1) != 1 and self.vocab_size > 1) or \
+        if out.get_device() != self._index or out.shape != (hidden.shape[0], self.vocab_size) or (out.stride(1) != 1 and self.vocab_size > 1) or \
                 (dtype is not None and out.dtype != dtype):
             raise SamplerError(_capi.INVALID_ARGUMENT, f"out must be [rows, {self.vocab_size}] on {self.device} with unit inner stride")
         return out

@@ -214,6 +214,8 @@ class Sampler:
         logits = head._output(hidden, logits, dtype)
         if out is None:
             out = torch.empty(hidden.shape[0], dtype=torch.int32, device=hidden.device)
+        elif out.device != hidden.device or out.dtype != torch.int32 or out.shape != hidden.shape[:1] or not out.is_contiguous():
+            raise SamplerError(_capi.INVALID_ARGUMENT, "out must be a contiguous int32 tensor [rows] next to the hidden states")
         stream = torch.cuda.current_stream(hidden.device).cuda_stream
         # (a tensor of one row may have any stride; the call wants one that holds the row)
         self._check(_capi.lib().ets_sampler_sample_hidden(
