@@ -19,6 +19,8 @@
 
 #include "ets_device.h"
 
+#include <type_traits>
+
 namespace ets {
 
 constexpr int kHeadBlock = 256;  // lanes of a workgroup
@@ -106,7 +108,7 @@ struct RawX {  // eight columns of x as they are in memory
   u32x4 v[XT == kDtypeFloat ? 2 : 1];
 };
 
-// Columns [k, k + 8) of a row; columns at `hidden` and behind, and rows that do not exist, read as 0.
+// Eight columns of a row from `at` on.
 template <int XT>
 __device__ __forceinline__ RawX<XT> load_whole_x(const char* at) {
   RawX<XT> out;
@@ -119,18 +121,18 @@ __device__ __forceinline__ RawX<XT> load_whole_x(const char* at) {
   }
   return out;
 }
+// ... the first of which is column k; columns at `hidden` and behind read as 0.
 template <int XT>
-__device__ __forceinline__ RawX<XT> load_raw_x(const char* row, int k, int hidden, bool exists) {
+__device__ __forceinline__ RawX<XT> load_raw_x(const char* at, int k, int hidden) {
   RawX<XT> out = {};
-  if (!exists) return out;
-  if (k + 8 <= hidden) return load_whole_x<XT>(row + static_cast<int64_t>(k) * ElemSize<XT>::value);
+  if (k + 8 <= hidden) return load_whole_x<XT>(at);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     if (k + j < hidden) {
       if (XT == kDtypeFloat) {
-        out.v[j >> 2][j & 3] = reinterpret_cast<const uint32_t*>(row)[k + j];
+        out.v[j >> 2][j & 3] = reinterpret_cast<const uint32_t*>(at)[j];
       } else {
-        out.v[0][j >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[k + j]) << (16 * (j & 1));
+        out.v[0][j >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(at)[j]) << (16 * (j & 1));
       }
     }
   }
@@ -167,21 +169,32 @@ __device__ __forceinline__ int chunk_group(const HeadParams& p, int chunk) {
   return p.chunks_per_group == 1 ? chunk : static_cast<int>(__umulhi(static_cast<uint32_t>(chunk), p.group_magic));
 }
 
-// The scales (or zeros) of this lane's vocabulary row for the GPC groups of a chunk.
+// The scales of a vocabulary row for a chunk's groups, as they are in memory: GPC of SB bytes.  `there`: all bits, or
+// none, which makes it 0.
 template <int GPC, int SB>
-__device__ __forceinline__ void load_scales(const void* base, const HeadParams& p, int tile, int chunk, int n, float* s) {
-  const int64_t at = ((static_cast<int64_t>(GPC > 1 ? chunk : chunk_group(p, chunk)) * p.tiles + tile) * kTileRows + n) * GPC;
-  if (SB == 4) {
-    struct alignas(4 * GPC) Raw { float f[GPC]; };
-    const Raw r = *reinterpret_cast<const Raw*>(static_cast<const float*>(base) + at);
-#pragma unroll
-    for (int g = 0; g < GPC; ++g) s[g] = r.f[g];
+struct RawScales {
+  uint32_t v[GPC * SB > 4 ? GPC * SB / 4 : 1];
+};
+template <int GPC, int SB>
+__device__ __forceinline__ RawScales<GPC, SB> load_raw_scales(const char* at) {
+  RawScales<GPC, SB> r;
+  if (GPC * SB == 2) {
+    r.v[0] = *reinterpret_cast<const uint16_t*>(at);
   } else {
-    struct alignas(2 * GPC) Raw { uint16_t u[GPC]; };
-    const Raw r = *reinterpret_cast<const Raw*>(static_cast<const uint16_t*>(base) + at);
+    struct alignas(GPC * SB > 2 ? GPC * SB : 4) Words { uint32_t v[GPC * SB > 4 ? GPC * SB / 4 : 1]; };
+    const Words w = *reinterpret_cast<const Words*>(at);
 #pragma unroll
-    for (int g = 0; g < GPC; ++g) s[g] = p.scale_is_bf16 ? __uint_as_float(static_cast<uint32_t>(r.u[g]) << 16) : half_bits_to_float(r.u[g]);
+    for (int i = 0; i < (GPC * SB > 4 ? GPC * SB / 4 : 1); ++i) r.v[i] = w.v[i];
   }
+  return r;
+}
+template <int GPC, int SB>
+__device__ __forceinline__ float scale_of(const RawScales<GPC, SB>& r, const HeadParams& p, int g, uint32_t there) {
+  if (SB == 4) return __uint_as_float(r.v[SB == 4 ? g : 0] & there);
+  const uint32_t pair = r.v[SB == 4 ? 0 : g >> 1], h = g & 1 ? pair >> 16 : pair & 0xffffu;
+  // (chosen by bits: a branch would wait for all loads in flight)
+  const uint32_t bf16 = 0u - static_cast<uint32_t>(p.scale_is_bf16);
+  return __uint_as_float((h << 16 & bf16 & there) | (__float_as_uint(half_bits_to_float(h)) & ~bf16 & there));
 }
 
 // The one rounding of the result, to nearest even.
@@ -257,45 +270,51 @@ head_stream_kernel(const HeadParams p) {
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, q = lane >> 4;
   const int tile0 = blockIdx.x * NT, m0 = blockIdx.y * 16;
   const int part = BESIDE ? n / kRowsBeside : 0, row = m0 + (BESIDE ? n % kRowsBeside : n);
-  const bool exists = row < p.rows && part < 3;
   const uint32_t first = part >= 1 ? 0xffff0000u : 0u, second = part >= 2 ? 0xffff0000u : 0u;
-  const char* x_row = static_cast<const char*>(p.x) + (exists ? row : 0) * p.x_stride * ElemSize<XT>::value;
-  const u32x4 minus24 = {M::kMinus24, M::kMinus24, M::kMinus24, M::kMinus24}, one = {M::kOne, M::kOne, M::kOne, M::kOne};
+  // (in the place of rows that do not exist the last one is multiplied again, and not stored)
+  const char* x_row = static_cast<const char*>(p.x) + min(row, p.rows - 1) * p.x_stride * ElemSize<XT>::value + 8 * q * ElemSize<XT>::value;
+  const u32x4 minus24 = {M::kMinus24, M::kMinus24, M::kMinus24, M::kMinus24};
   const uint32_t unpack_base = base_in_register<XT>();
   f32x4 total[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) total[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  for (int chunk = wave; chunk < p.chunks; chunk += kWavesHere) {
+  auto add_chunk = [&](int chunk, auto whole) {
     u32x4 w[NT];
-    float s[NT][GPC], z[NT][GPC];
+    RawScales<GPC, SB> s[NT], z[NT];
+    RawX<XT> raw[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int k = chunk * kChunkCols + 32 * t;  // (the lane's part of the column is in x_row)
+      const char* from = x_row + static_cast<int64_t>(k) * ElemSize<XT>::value;
+      raw[t] = whole.value ? load_whole_x<XT>(from) : load_raw_x<XT>(from, k + 8 * q, p.hidden);
+    }
+    const int64_t block0 = static_cast<int64_t>(chunk) * p.tiles;
+    const int64_t scale0 = GPC > 1 ? block0 : static_cast<int64_t>(chunk_group(p, chunk)) * p.tiles;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int tile = min(tile0 + i, p.tiles - 1);  // (tiles behind the last one are computed again and not stored)
-      w[i] = p.blocks[(static_cast<int64_t>(chunk) * p.tiles + tile) * 64 + lane];
-      load_scales<GPC, SB>(p.scales, p, tile, chunk, n, s[i]);
-      if (ZEROS) load_scales<GPC, SB>(p.zeros, p, tile, chunk, n, z[i]);
+      w[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p.blocks) + (block0 + tile) * 1024 + static_cast<uint32_t>(lane * 16));
+      const int64_t scale_at = (scale0 + tile) * (kTileRows * GPC * SB);
+      s[i] = load_raw_scales<GPC, SB>(static_cast<const char*>(p.scales) + scale_at + static_cast<uint32_t>(n * (GPC * SB)));
+      if (ZEROS) z[i] = load_raw_scales<GPC, SB>(static_cast<const char*>(p.zeros) + scale_at + static_cast<uint32_t>(n * (GPC * SB)));
     }
     u32x4 x[4][P];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const RawX<XT> raw = load_raw_x<XT>(x_row, chunk * kChunkCols + 32 * t + 8 * q, p.hidden, exists);
       if constexpr (BESIDE) {
-        x[t][0] = part_of_x(raw, first, second);
+        x[t][0] = part_of_x(raw[t], first, second);
       } else {
-        split_x<XT>(raw, x[t]);
+        split_x<XT>(raw[t], x[t]);
       }
     }
 #pragma unroll
     for (int g = 0; g < GPC; ++g) {
-      f32x4 base = {0.0f, 0.0f, 0.0f, 0.0f}, sums = {0.0f, 0.0f, 0.0f, 0.0f};
+      f32x4 base = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int t = g * kSteps; t < (g + 1) * kSteps; ++t) {
 #pragma unroll
-        for (int k = 0; k < P; ++k) {
-          base = M::product(x[t][k], minus24, base);
-          if (ZEROS) sums = M::product(x[t][k], one, sums);
-        }
+        for (int k = 0; k < P; ++k) base = M::product(x[t][k], minus24, base);
       }
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
@@ -306,14 +325,21 @@ head_stream_kernel(const HeadParams p) {
 #pragma unroll
           for (int k = 0; k < P; ++k) acc = M::product(x[t][k], b, acc);
         }
+        const float scale = scale_of<GPC, SB>(s[i], p, g, ~0u);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          total[i][r] = fmaf(s[i][g], acc[r], total[i][r]);
-          if (ZEROS) total[i][r] = fmaf(z[i][g], sums[r], total[i][r]);
+        for (int r = 0; r < 4; ++r) total[i][r] = fmaf(scale, acc[r], total[i][r]);
+        if (ZEROS) {
+          const float zero = scale_of<GPC, SB>(z[i], p, g, ~0u) * (-1.0f / 24.0f);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) total[i][r] = fmaf(zero, base[r], total[i][r]);
         }
       }
     }
-  }
+  };
+  const int whole_chunks = p.hidden / kChunkCols;
+  int chunk = wave;
+  for (; chunk < whole_chunks; chunk += kWavesHere) add_chunk(chunk, std::true_type{});
+  if (chunk < p.chunks) add_chunk(chunk, std::false_type{});
 #pragma unroll
   for (int i = 0; i < NT; ++i) *reinterpret_cast<f32x4*>(&red[wave][i][lane * 4]) = total[i];
   __syncthreads();
@@ -384,7 +410,8 @@ head_rows_kernel(const void* x, int64_t x_stride, int32_t rows, int32_t hidden, 
   const int slot = threadIdx.x & 15, in_tile = threadIdx.x >> 4, chunk = blockIdx.x, m = blockIdx.y * 16 + in_tile;
   const bool exists = m < rows;
   const char* row = static_cast<const char*>(x) + (exists ? m : 0) * x_stride * ElemSize<XT>::value;
-  const RawX<XT> raw = load_raw_x<XT>(row, chunk * kChunkCols + 8 * slot, hidden, exists);
+  const int k = chunk * kChunkCols + 8 * slot;
+  const RawX<XT> raw = load_raw_x<XT>(row + static_cast<int64_t>(k) * ElemSize<XT>::value, k, exists ? hidden : 0);
   u32x4 part[P];
   split_x<XT>(raw, part);
   const int64_t block = static_cast<int64_t>(blockIdx.y) * gridDim.x + chunk;
@@ -396,34 +423,6 @@ head_rows_kernel(const void* x, int64_t x_stride, int32_t rows, int32_t hidden, 
   if (GPC <= 2) s = dpp_add<0x141>(s);
   if (GPC == 1) s = dpp_add<0x140>(s);
   if (slot % (16 / GPC) == 0) sums[(block * GPC + slot / (16 / GPC)) * 16 + in_tile] = s;
-}
-
-// The scales of a vocabulary row for a chunk's groups, as they are in memory: GPC of SB bytes.  `there`: all bits, or
-// none, which makes it 0.
-template <int GPC, int SB>
-struct RawScales {
-  uint32_t v[GPC * SB > 4 ? GPC * SB / 4 : 1];
-};
-template <int GPC, int SB>
-__device__ __forceinline__ RawScales<GPC, SB> load_raw_scales(const char* at) {
-  RawScales<GPC, SB> r;
-  if (GPC * SB == 2) {
-    r.v[0] = *reinterpret_cast<const uint16_t*>(at);
-  } else {
-    struct alignas(GPC * SB > 2 ? GPC * SB : 4) Words { uint32_t v[GPC * SB > 4 ? GPC * SB / 4 : 1]; };
-    const Words w = *reinterpret_cast<const Words*>(at);
-#pragma unroll
-    for (int i = 0; i < (GPC * SB > 4 ? GPC * SB / 4 : 1); ++i) r.v[i] = w.v[i];
-  }
-  return r;
-}
-template <int GPC, int SB>
-__device__ __forceinline__ float scale_of(const RawScales<GPC, SB>& r, const HeadParams& p, int g, uint32_t there) {
-  if (SB == 4) return __uint_as_float(r.v[SB == 4 ? g : 0] & there);
-  const uint32_t pair = r.v[SB == 4 ? 0 : g >> 1], h = g & 1 ? pair >> 16 : pair & 0xffffu;
-  // (chosen by bits: a branch would wait for all loads in flight)
-  const uint32_t bf16 = 0u - static_cast<uint32_t>(p.scale_is_bf16);
-  return __uint_as_float((h << 16 & bf16 & there) | (__float_as_uint(half_bits_to_float(h)) & ~bf16 & there));
 }
 
 template <int XT, int GPC, int SB, bool ZEROS, int MT, int NT, int WV, int WK>
