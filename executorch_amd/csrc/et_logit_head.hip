@@ -53,7 +53,6 @@ struct ets_logit_head {
   int device = 0;
   int32_t tiles = 0, chunks = 0, chunks_per_group = 1, groups = 0;
   ets_host::HeadForm form = {};
-  bool scale_is_bf16 = false;
   void* d_blocks = nullptr;
   void* d_scales = nullptr;
   void* d_zeros = nullptr;
@@ -116,9 +115,8 @@ ets_status ets_logit_head_create(int32_t vocab_size, int32_t hidden_size, int32_
   h->tiles = (vocab_size + ets::kTileRows - 1) / ets::kTileRows;
   h->chunks = (hidden_size + ets::kChunkCols - 1) / ets::kChunkCols;
   h->form.groups_per_chunk = group_size < ets::kChunkCols ? ets::kChunkCols / group_size : 1;
-  h->form.scale_bytes = static_cast<int>(scale_bytes);
+  h->form.scale_type = scale_dtype;
   h->form.zeros = d_zeros != nullptr;
-  h->scale_is_bf16 = scale_dtype == ETS_DTYPE_BFLOAT16;
   h->chunks_per_group = group_size < ets::kChunkCols ? 1 : std::min(group_size / ets::kChunkCols, h->chunks);
   const int32_t groups = (hidden_size - 1) / group_size + 1;  // of a row, as the caller has them
   h->groups = groups;
@@ -198,8 +196,6 @@ ets_status ets_logit_head_logits(ets_logit_head* h, const void* d_hidden, int32_
   p.blocks = static_cast<const ets::u32x4*>(h->d_blocks);
   p.scales = h->d_scales;
   p.zeros = h->d_zeros;
-  p.scale_bytes = h->form.scale_bytes;
-  p.scale_is_bf16 = h->scale_is_bf16;
   p.tiles = h->tiles;
   p.chunks = h->chunks;
   p.chunks_per_group = h->chunks_per_group;

@@ -8,7 +8,7 @@ namespace ets_host {
 // How the weights are laid out: what picks an instantiation besides the hidden states' type.
 struct HeadForm {
   int groups_per_chunk;  // 4, 2 or 1
-  int scale_bytes;       // 4 or 2
+  int32_t scale_type;    // element type of scales and zeros
   bool zeros;
 };
 
@@ -19,48 +19,48 @@ hipError_t launch_head_f32(const ets::HeadParams& p, const HeadForm& f, hipStrea
 hipError_t launch_head_f16(const ets::HeadParams& p, const HeadForm& f, hipStream_t stream);
 hipError_t launch_head_bf16(const ets::HeadParams& p, const HeadForm& f, hipStream_t stream);
 
-template <int XT, int GPC, int SB, bool ZEROS, int NT, bool BESIDE>
+template <int XT, int GPC, int ST, bool ZEROS, int NT, bool BESIDE>
 hipError_t launch_stream(const ets::HeadParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL((ets::head_stream_kernel<XT, GPC, SB, ZEROS, NT, BESIDE>), dim3((p.tiles + NT - 1) / NT),
+  hipLaunchKernelGGL((ets::head_stream_kernel<XT, GPC, ST, ZEROS, NT, BESIDE>), dim3((p.tiles + NT - 1) / NT),
                      dim3(ets::kHeadBlock), 0, stream, p);
   return hipGetLastError();
 }
 
-template <int XT, int GPC, int SB, bool ZEROS, int NT>
+template <int XT, int GPC, int ST, bool ZEROS, int NT>
 hipError_t launch_stream(const ets::HeadParams& p, hipStream_t stream) {
   if constexpr (XT == ets::kDtypeFloat) {
-    if (p.rows <= ets::kRowsBeside) return launch_stream<XT, GPC, SB, ZEROS, NT, true>(p, stream);
+    if (p.rows <= ets::kRowsBeside) return launch_stream<XT, GPC, ST, ZEROS, NT, true>(p, stream);
   }
-  return launch_stream<XT, GPC, SB, ZEROS, NT, false>(p, stream);
+  return launch_stream<XT, GPC, ST, ZEROS, NT, false>(p, stream);
 }
 
-template <int XT, int GPC, int SB, bool ZEROS>
+template <int XT, int GPC, int ST, bool ZEROS>
 hipError_t launch_head(const ets::HeadParams& p, hipStream_t stream) {
   // Four tiles a workgroup where that makes four workgroups for each of the 256 CUs, otherwise two (2000 tiles of 2048
   // columns: 9.2 us against 10.3; 8016 tiles of 4096: 53 us against 49).  Of fp32 hidden states a workgroup reads so
   // much that it is four always (3142 tiles of 1601 columns: 17 us against 20).
-  if (XT == ets::kDtypeFloat || p.tiles >= 4096) return launch_stream<XT, GPC, SB, ZEROS, 4>(p, stream);
-  return launch_stream<XT, GPC, SB, ZEROS, XT == ets::kDtypeFloat ? 4 : 2>(p, stream);
+  if (XT == ets::kDtypeFloat || p.tiles >= 4096) return launch_stream<XT, GPC, ST, ZEROS, 4>(p, stream);
+  return launch_stream<XT, GPC, ST, ZEROS, XT == ets::kDtypeFloat ? 4 : 2>(p, stream);
 }
 
-template <int XT, int GPC, int SB, bool ZEROS, int MT, int NT, int WV, int WK>
+template <int XT, int GPC, int ST, bool ZEROS, int MT, int NT, int WV, int WK>
 hipError_t launch_tiles(const ets::HeadParams& p, hipStream_t stream) {
   const int64_t vocab_blocks = (p.tiles + WV * NT - 1) / (WV * NT), row_blocks = (p.rows + 16 * MT - 1) / (16 * MT);
-  hipLaunchKernelGGL((ets::head_tile_kernel<XT, GPC, SB, ZEROS, MT, NT, WV, WK>),
+  hipLaunchKernelGGL((ets::head_tile_kernel<XT, GPC, ST, ZEROS, MT, NT, WV, WK>),
                      dim3(static_cast<uint32_t>((vocab_blocks + 7) / 8 * 8 * row_blocks)), dim3(64 * WV * WK), 0, stream, p);
   return hipGetLastError();
 }
 
-template <int XT, int GPC, int SB, bool ZEROS, int MT>
+template <int XT, int GPC, int ST, bool ZEROS, int MT>
 hipError_t launch_tiles(const ets::HeadParams& p, hipStream_t stream) {
   // 512 vocabulary entries a workgroup where that makes at least one for nearly each of the 256 CUs; otherwise 128, with
   // two waves behind each other along the columns.
-  return p.tiles >= 240 * 32 ? launch_tiles<XT, GPC, SB, ZEROS, MT, 4, 8, 1>(p, stream) : launch_tiles<XT, GPC, SB, ZEROS, MT, 2, 4, 2>(p, stream);
+  return p.tiles >= 240 * 32 ? launch_tiles<XT, GPC, ST, ZEROS, MT, 4, 8, 1>(p, stream) : launch_tiles<XT, GPC, ST, ZEROS, MT, 2, 4, 2>(p, stream);
 }
 
-template <int XT, int GPC, int SB, bool ZEROS>
+template <int XT, int GPC, int ST, bool ZEROS>
 hipError_t launch_head_rows(const ets::HeadParams& whole, hipStream_t stream) {
-  if (whole.rows <= 16) return launch_head<XT, GPC, SB, ZEROS>(whole, stream);
+  if (whole.rows <= 16) return launch_head<XT, GPC, ST, ZEROS>(whole, stream);
   constexpr int kRowsAtOnce = kWorkTiles / ets::Parts<XT>::value / 2 * 2 * 16;  // as the work buffer holds
   const int32_t chunks = ets::padded_chunks(whole.chunks);
   for (int32_t row = 0; row < whole.rows; row += kRowsAtOnce) {
@@ -72,8 +72,17 @@ hipError_t launch_head_rows(const ets::HeadParams& whole, hipStream_t stream) {
                        const_cast<ets::u32x4*>(p.units), const_cast<float*>(reinterpret_cast<const float*>(p.sums)));
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    e = p.rows <= 32 || XT == ets::kDtypeFloat ? launch_tiles<XT, GPC, SB, ZEROS, 2>(p, stream)
-                                               : launch_tiles<XT, GPC, SB, ZEROS, XT == ets::kDtypeFloat ? 2 : 4>(p, stream);
+    // Workgroups of four 16-row tiles, or of three where that makes no more of them (37 rows at 32000 x 4096: 26.6 us
+    // instead of 30.7); of two for up to 32 rows and for fp32, whose three parts take the registers.
+    const int32_t row_tiles = (p.rows + 15) / 16;
+    if constexpr (XT == ets::kDtypeFloat) {
+      e = launch_tiles<XT, GPC, ST, ZEROS, 2>(p, stream);
+    } else if (row_tiles <= 2) {
+      e = launch_tiles<XT, GPC, ST, ZEROS, 2>(p, stream);
+    } else {
+      e = (row_tiles + 2) / 3 == (row_tiles + 3) / 4 ? launch_tiles<XT, GPC, ST, ZEROS, 3>(p, stream)
+                                                     : launch_tiles<XT, GPC, ST, ZEROS, 4>(p, stream);
+    }
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
@@ -81,7 +90,11 @@ hipError_t launch_head_rows(const ets::HeadParams& whole, hipStream_t stream) {
 
 template <int XT, int GPC, bool ZEROS>
 hipError_t launch_head(const ets::HeadParams& p, const HeadForm& f, hipStream_t stream) {
-  return f.scale_bytes == 4 ? launch_head_rows<XT, GPC, 4, ZEROS>(p, stream) : launch_head_rows<XT, GPC, 2, ZEROS>(p, stream);
+  switch (f.scale_type) {
+    case ets::kDtypeFloat: return launch_head_rows<XT, GPC, ets::kDtypeFloat, ZEROS>(p, stream);
+    case ets::kDtypeHalf: return launch_head_rows<XT, GPC, ets::kDtypeHalf, ZEROS>(p, stream);
+    default: return launch_head_rows<XT, GPC, ets::kDtypeBFloat16, ZEROS>(p, stream);
+  }
 }
 
 template <int XT, int GPC>

@@ -37,8 +37,6 @@ struct HeadParams {
   const u32x4* blocks;  // [chunks, tiles, 64]
   const void* scales;   // [chunks, tiles, 16, groups per chunk], or [groups, tiles, 16] for groups of 128 columns and more
   const void* zeros;    // the same, or null
-  int32_t scale_bytes;    // 4 (fp32) or 2
-  int32_t scale_is_bf16;  // of 16-bit scales: bf16, else fp16
   int32_t tiles, chunks, chunks_per_group, groups;  // (the last two for groups of 128 columns and more)
   uint32_t group_magic;   // ceil(2^32 / chunks_per_group): the upper word of chunk x group_magic is the chunk's group
   int32_t vocab, hidden, rows;
@@ -169,32 +167,33 @@ __device__ __forceinline__ int chunk_group(const HeadParams& p, int chunk) {
   return p.chunks_per_group == 1 ? chunk : static_cast<int>(__umulhi(static_cast<uint32_t>(chunk), p.group_magic));
 }
 
-// The scales of a vocabulary row for a chunk's groups, as they are in memory: GPC of SB bytes.  `there`: all bits, or
-// none, which makes it 0.
-template <int GPC, int SB>
+// The scales of a vocabulary row for a chunk's groups, as they are in memory: GPC of the type ST.
+template <int GPC, int ST>
 struct RawScales {
-  uint32_t v[GPC * SB > 4 ? GPC * SB / 4 : 1];
+  static constexpr int kBytes = GPC * ElemSize<ST>::value, kWords = kBytes > 4 ? kBytes / 4 : 1;
+  uint32_t v[kWords];
 };
-template <int GPC, int SB>
-__device__ __forceinline__ RawScales<GPC, SB> load_raw_scales(const char* at) {
-  RawScales<GPC, SB> r;
-  if (GPC * SB == 2) {
+template <int GPC, int ST>
+__device__ __forceinline__ RawScales<GPC, ST> load_raw_scales(const char* at) {
+  using Raw = RawScales<GPC, ST>;
+  Raw r;
+  if (Raw::kBytes == 2) {
     r.v[0] = *reinterpret_cast<const uint16_t*>(at);
   } else {
-    struct alignas(GPC * SB > 2 ? GPC * SB : 4) Words { uint32_t v[GPC * SB > 4 ? GPC * SB / 4 : 1]; };
+    struct alignas(Raw::kBytes > 2 ? Raw::kBytes : 4) Words { uint32_t v[Raw::kWords]; };
     const Words w = *reinterpret_cast<const Words*>(at);
 #pragma unroll
-    for (int i = 0; i < (GPC * SB > 4 ? GPC * SB / 4 : 1); ++i) r.v[i] = w.v[i];
+    for (int i = 0; i < Raw::kWords; ++i) r.v[i] = w.v[i];
   }
   return r;
 }
-template <int GPC, int SB>
-__device__ __forceinline__ float scale_of(const RawScales<GPC, SB>& r, const HeadParams& p, int g, uint32_t there) {
-  if (SB == 4) return __uint_as_float(r.v[SB == 4 ? g : 0] & there);
-  const uint32_t pair = r.v[SB == 4 ? 0 : g >> 1], h = g & 1 ? pair >> 16 : pair & 0xffffu;
-  // (chosen by bits: a branch would wait for all loads in flight)
-  const uint32_t bf16 = 0u - static_cast<uint32_t>(p.scale_is_bf16);
-  return __uint_as_float((h << 16 & bf16 & there) | (__float_as_uint(half_bits_to_float(h)) & ~bf16 & there));
+// `there`: all bits, or none, which makes it 0.
+template <int GPC, int ST>
+__device__ __forceinline__ float scale_of(const RawScales<GPC, ST>& r, int g, uint32_t there) {
+  if (ST == kDtypeFloat) return __uint_as_float(r.v[ST == kDtypeFloat ? g : 0] & there);
+  const uint32_t pair = r.v[ST == kDtypeFloat ? 0 : g >> 1];
+  if (ST == kDtypeBFloat16) return __uint_as_float((g & 1 ? pair & 0xffff0000u : pair << 16) & there);
+  return __uint_as_float(__float_as_uint(half_bits_to_float((g & 1 ? pair >> 16 : pair) & 0xffffu)) & there);
 }
 
 // The one rounding of the result, to nearest even.
@@ -256,12 +255,12 @@ __device__ __forceinline__ u32x4 part_of_x(const RawX<kDtypeFloat>& x, uint32_t 
 // and their sums are added up in a fixed order at the end.  BESIDE, for up to five rows of fp32: the parts of a row
 // are three rows of the same operand, 5 apart, instead of three operands.
 //
-// Bound by the reads of the weights: 128256 x 4096 in groups of 128, 272 MB, in 49 us, 5.5 TB/s, where a kernel that
-// only reads reaches 5.95 TB/s.  x comes from the caches for every NT tiles again, which is what holds back fp32 (50257 x
-// 1601, 3 rows: 3.1 TB/s; 20 us with an operand for each part).  No copy of the next chunk's weights in a second set
-// of registers: it halves the waves on a SIMD and is slower everywhere (128256 x 4096: 51 us; 151936 x 5120 with
-// zeros: 105 us instead of 93).
-template <int XT, int GPC, int SB, bool ZEROS, int NT, bool BESIDE>
+// Bound by the reads of the weights: 128256 x 4096 in groups of 128, 272 MB, in 47.6 us, 5.7 TB/s, where a kernel that
+// only reads reaches 5.95 TB/s; 151936 x 5120 in groups of 64 with zeros, 440 MB, in 83 us, 5.3 TB/s.  x comes from the
+// caches for every NT tiles again, which is what holds back fp32 (50257 x 1601, 3 rows: 16 us, 3.1 TB/s; 20 us with an
+// operand for each part).  No copy of the next chunk's weights in a second set of registers: it halves the waves on a
+// SIMD and is slower everywhere (128256 x 4096: 51 us; 151936 x 5120 with zeros: 105 us).
+template <int XT, int GPC, int ST, bool ZEROS, int NT, bool BESIDE>
 __global__ void __launch_bounds__(kHeadBlock)
 head_stream_kernel(const HeadParams p) {
   using M = Matrix<XT>;
@@ -281,7 +280,7 @@ head_stream_kernel(const HeadParams p) {
 
   auto add_chunk = [&](int chunk, auto whole) {
     u32x4 w[NT];
-    RawScales<GPC, SB> s[NT], z[NT];
+    RawScales<GPC, ST> s[NT], z[NT];
     RawX<XT> raw[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -295,9 +294,9 @@ head_stream_kernel(const HeadParams p) {
     for (int i = 0; i < NT; ++i) {
       const int tile = min(tile0 + i, p.tiles - 1);  // (tiles behind the last one are computed again and not stored)
       w[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p.blocks) + (block0 + tile) * 1024 + static_cast<uint32_t>(lane * 16));
-      const int64_t scale_at = (scale0 + tile) * (kTileRows * GPC * SB);
-      s[i] = load_raw_scales<GPC, SB>(static_cast<const char*>(p.scales) + scale_at + static_cast<uint32_t>(n * (GPC * SB)));
-      if (ZEROS) z[i] = load_raw_scales<GPC, SB>(static_cast<const char*>(p.zeros) + scale_at + static_cast<uint32_t>(n * (GPC * SB)));
+      const int64_t scale_at = (scale0 + tile) * (kTileRows * GPC * ElemSize<ST>::value);
+      s[i] = load_raw_scales<GPC, ST>(static_cast<const char*>(p.scales) + scale_at + static_cast<uint32_t>(n * (GPC * ElemSize<ST>::value)));
+      if (ZEROS) z[i] = load_raw_scales<GPC, ST>(static_cast<const char*>(p.zeros) + scale_at + static_cast<uint32_t>(n * (GPC * ElemSize<ST>::value)));
     }
     u32x4 x[4][P];
 #pragma unroll
@@ -325,11 +324,11 @@ head_stream_kernel(const HeadParams p) {
 #pragma unroll
           for (int k = 0; k < P; ++k) acc = M::product(x[t][k], b, acc);
         }
-        const float scale = scale_of<GPC, SB>(s[i], p, g, ~0u);
+        const float scale = scale_of<GPC, ST>(s[i], g, ~0u);
 #pragma unroll
         for (int r = 0; r < 4; ++r) total[i][r] = fmaf(scale, acc[r], total[i][r]);
         if (ZEROS) {
-          const float zero = scale_of<GPC, SB>(z[i], p, g, ~0u) * (-1.0f / 24.0f);
+          const float zero = scale_of<GPC, ST>(z[i], g, ~0u) * (-1.0f / 24.0f);
 #pragma unroll
           for (int r = 0; r < 4; ++r) total[i][r] = fmaf(zero, base[r], total[i][r]);
         }
@@ -425,17 +424,17 @@ head_rows_kernel(const void* x, int64_t x_stride, int32_t rows, int32_t hidden, 
   if (slot % (16 / GPC) == 0) sums[(block * GPC + slot / (16 / GPC)) * 16 + in_tile] = s;
 }
 
-template <int XT, int GPC, int SB, bool ZEROS, int MT, int NT, int WV, int WK>
+template <int XT, int GPC, int ST, bool ZEROS, int MT, int NT, int WV, int WK>
 __global__ void __launch_bounds__(64 * WV * WK, 2)
 head_tile_kernel(const HeadParams p) {
   using M = Matrix<XT>;
   constexpr int P = Parts<XT>::value, kSteps = 4 / GPC, kLanes = 64 * WV * WK, kRows = 16 * MT;
   constexpr int kUnits = WK * P * MT * 256;  // of x per step
-  constexpr int kCopies = kUnits / kLanes;   // of them per lane
+  constexpr int kCopies = (kUnits + kLanes - 1) / kLanes, kPlaces = kCopies * kLanes;  // of them per lane; with those too many
   constexpr int kSums = WK * MT * GPC * 4;   // quadruples of row sums per step
-  static_assert(kUnits % kLanes == 0 && kSums <= kLanes, "");
+  static_assert(kPlaces < 2 * kUnits && kUnits % 64 == 0 && kSums <= kLanes, "");
   constexpr int kOut = WK * WV * 16 * NT * 16;  // floats of 16 rows of the result, per wave
-  constexpr int kBytes = 2 * kUnits * 16 > kOut * 4 ? 2 * kUnits * 16 : kOut * 4;
+  constexpr int kBytes = 2 * kPlaces * 16 > kOut * 4 ? 2 * kPlaces * 16 : kOut * 4;
   __shared__ __attribute__((aligned(16))) char lds[kBytes];
   __shared__ f32x4 sums_lds[2][kSums];
   u32x4* units = reinterpret_cast<u32x4*>(lds);
@@ -453,7 +452,7 @@ head_tile_kernel(const HeadParams p) {
   static_assert(kChunkRound % (2 * WK) == 0, "whole rounds of two steps");
   u32x4 x_raw[kCopies], w_raw[NT];
   f32x4 sums_raw;
-  RawScales<GPC, SB> s_raw[NT], z_raw[NT];
+  RawScales<GPC, ST> s_raw[NT], z_raw[NT];
   // Unit u of a step: chunk u / (256 P MT) of it, 16-row tile u / (256 P) % MT (of those that do not exist the last one).
   // Everything but the lane's offset is the same in every lane of a wave.
   const int work_chunks = padded_chunks(p.chunks);
@@ -463,7 +462,8 @@ head_tile_kernel(const HeadParams p) {
   auto load_step_x = [&](int step) {
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
-      const int u = i * kLanes + wave * 64, tile = min(row_block * MT + u / (256 * P) % MT, row_tiles - 1);
+      const int place = i * kLanes + wave * 64, u = kPlaces == kUnits || place < kUnits ? place : place - kUnits;  // (those too many: the first again)
+      const int tile = min(row_block * MT + u / (256 * P) % MT, row_tiles - 1);
       const int64_t unit = (static_cast<int64_t>(tile) * work_chunks + step * WK + u / (256 * P * MT)) * (256 * P) + u % (256 * P);
       x_raw[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p.units) + unit * 16 + static_cast<uint32_t>(lane * 16));
     }
@@ -471,7 +471,7 @@ head_tile_kernel(const HeadParams p) {
   };
   auto store_step_x = [&](int buffer) {
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) units[buffer * kUnits + i * kLanes + tid] = x_raw[i];
+    for (int i = 0; i < kCopies; ++i) units[buffer * kPlaces + i * kLanes + tid] = x_raw[i];
     sums_lds[buffer][sum_u] = sums_raw;
   };
   // (all of these offsets but the lane's are the same in every lane)
@@ -484,10 +484,10 @@ head_tile_kernel(const HeadParams p) {
       const int tile = min(tile0 + i, p.tiles - 1);
       w_raw[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p.blocks) + (block0 + tile) * 1024 +
                                                        static_cast<uint32_t>(lane * 16));
-      const int64_t scale_at = (scale0 + tile) * (kTileRows * GPC * SB);
-      s_raw[i] = load_raw_scales<GPC, SB>(static_cast<const char*>(p.scales) + scale_at + static_cast<uint32_t>(n * (GPC * SB)));
+      const int64_t scale_at = (scale0 + tile) * (kTileRows * GPC * ElemSize<ST>::value);
+      s_raw[i] = load_raw_scales<GPC, ST>(static_cast<const char*>(p.scales) + scale_at + static_cast<uint32_t>(n * (GPC * ElemSize<ST>::value)));
       if (ZEROS)
-        z_raw[i] = load_raw_scales<GPC, SB>(static_cast<const char*>(p.zeros) + scale_at + static_cast<uint32_t>(n * (GPC * SB)));
+        z_raw[i] = load_raw_scales<GPC, ST>(static_cast<const char*>(p.zeros) + scale_at + static_cast<uint32_t>(n * (GPC * ElemSize<ST>::value)));
     }
   };
 
@@ -522,7 +522,7 @@ head_tile_kernel(const HeadParams p) {
         if (t == 0) base[stage % kBases] = sums_lds[buffer][((wk * MT + a) * GPC + g) * 4 + q];
 #pragma unroll
         for (int c = 0; c < P; ++c)
-          x[at % (kReads + 1)][c] = units[buffer * kUnits + ((wk * MT + a) * P + c) * 256 + (g * kSteps + t) * 64 + lane];
+          x[at % (kReads + 1)][c] = units[buffer * kPlaces + ((wk * MT + a) * P + c) * 256 + (g * kSteps + t) * 64 + lane];
       };
       auto scale_rows = [&](int stage) {
         const int a = stage % MT;
@@ -543,8 +543,8 @@ head_tile_kernel(const HeadParams p) {
         if (a == 0) {
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
-            sc[i] = scale_of<GPC, SB>(s_raw[i], p, g, there);
-            if (ZEROS) zero[i] = scale_of<GPC, SB>(z_raw[i], p, g, there) * (-1.0f / 24.0f);
+            sc[i] = scale_of<GPC, ST>(s_raw[i], g, there);
+            if (ZEROS) zero[i] = scale_of<GPC, ST>(z_raw[i], g, there) * (-1.0f / 24.0f);
           }
         }
 #pragma unroll
