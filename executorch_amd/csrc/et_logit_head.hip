@@ -21,13 +21,20 @@ head_layout_kernel(const uint8_t* packed, int64_t stride, int32_t vocab, int32_t
     const int64_t block = d >> 8, chunk = block / tiles;
     const int64_t v = (block - chunk * tiles) * kTileRows + (lane & 15);
     const int k = static_cast<int>(chunk) * kChunkCols + 32 * t + 8 * (lane >> 4);
+    uint32_t from = 0x88888888u;  // eight columns as they are in memory, nibble j at bits 4 j
+    if (v < vocab && k + 8 <= hidden) {
+      struct __attribute__((packed, aligned(1))) Loose { uint32_t w; };
+      from = reinterpret_cast<const Loose*>(packed + v * stride + (k >> 1))->w;
+    } else if (v < vocab) {
+      for (int j = 0; j < 8 && k + j < hidden; ++j) {
+        const uint32_t nibble = (packed[v * stride + ((k + j) >> 1)] >> (4 * (j & 1))) & 15u;
+        from = (from & ~(15u << (4 * j))) | nibble << (4 * j);
+      }
+    }
     uint32_t w = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t nibble = 8;
-      if (v < vocab && k + j < hidden) nibble = (packed[v * stride + ((k + j) >> 1)] >> (4 * (j & 1))) & 15u;
-      w |= nibble << (16 * (j & 1) + 4 * (j >> 1));
-    }
+    for (int j = 0; j < 8; ++j) w |= (from >> (4 * j) & 15u) << (16 * (j & 1) + 4 * (j >> 1));
+    w = w << ets::kRotation | w >> (32 - ets::kRotation);
     blocks[d] = w;
   }
 }
@@ -128,7 +135,8 @@ ets_status ets_logit_head_create(int32_t vocab_size, int32_t hidden_size, int32_
   hipError_t e = hipGetDevice(&h->device);
   if (e != hipSuccess) return bail(e, "ets_logit_head_create: hipGetDevice");
   hipStream_t stream = static_cast<hipStream_t>(hip_stream);
-  const int64_t dwords = static_cast<int64_t>(h->tiles) * h->chunks * 256;
+  // (head_tile reads whole workgroups of tiles, behind a chunk's last tile the next chunk's and in the end this padding)
+  const int64_t dwords = (static_cast<int64_t>(h->tiles) * h->chunks + ets::kTilePadding) * 256;
   e = hipMalloc(&h->d_blocks, dwords * 4);
   if (e != hipSuccess) return bail(e, "ets_logit_head_create: hipMalloc(weights)");
   hipLaunchKernelGGL(ets::head_layout_kernel, dim3(layout_grid(dwords)), dim3(ets::kHeadBlock), 0, stream,
@@ -137,7 +145,7 @@ ets_status ets_logit_head_create(int32_t vocab_size, int32_t hidden_size, int32_
   e = hipGetLastError();
   if (e != hipSuccess) return bail(e, "ets_logit_head_create: launch");
   const int32_t per_chunk = h->form.groups_per_chunk;
-  const int64_t count = static_cast<int64_t>(ets::kTileRows) * h->tiles * (per_chunk > 1 ? h->chunks * per_chunk : groups);
+  const int64_t count = ets::kTileRows * (static_cast<int64_t>(h->tiles) * (per_chunk > 1 ? h->chunks : groups) + ets::kTilePadding) * per_chunk;
   for (int k = 0; k < (d_zeros ? 2 : 1); ++k) {
     void** dst = k ? &h->d_zeros : &h->d_scales;
     const void* src = k ? d_zeros : d_scales;

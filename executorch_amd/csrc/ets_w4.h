@@ -11,8 +11,8 @@
 //
 // Weight layout: blocks of 16 vocabulary rows x 128 columns, 1 KiB, the 16 bytes of a lane next to each
 // other: lane (q, n) = 16 q + n holds row n of the block, its dword t the columns 32 t + 8 q + 0..7 (operand
-// B of the t-th 16x16x32 product), the column 8 q + 2 i + h at bits 16 h + 4 i.  A wave reads a block with
-// one 16-byte load per lane.  The blocks of one chunk of columns are next to each other: workgroups that walk
+// B of the t-th 16x16x32 product), the column 8 q + 2 i + h at bits 16 h + 4 i + 3, around the end of the dword: with
+// bf16 two of its weights are then in place without a shift.  A wave reads a block with one 16-byte load per lane.  The blocks of one chunk of columns are next to each other: workgroups that walk
 // along the columns side by side then read one contiguous stretch of memory at a time, where blocks in row order
 // (32 KiB apart at 4096 columns) would have all of them at the same memory channels (64 rows: 134 us).
 #pragma once
@@ -26,6 +26,8 @@ namespace ets {
 constexpr int kHeadBlock = 256;  // lanes of a workgroup
 constexpr int kTileRows = 16;    // vocabulary rows of a block
 constexpr int kChunkCols = 128;  // columns of a block
+constexpr int kRotation = 3;     // of the packed words, to the left
+constexpr int kTilePadding = 32; // blocks behind the last one: a workgroup of head_tile takes up to as many at once
 constexpr int kRowsBeside = 5;   // rows of fp32 whose three parts fit one operand of 16 rows
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -83,8 +85,9 @@ __device__ __forceinline__ u32x4 unpack(uint32_t w, uint32_t base) {
   u32x4 b;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int shift = 4 * i - M::kTop;
-    b[i] = ((shift < 0 ? w << -shift : w >> shift) & M::kMask) | base;
+    const int right = 4 * i + kRotation - M::kTop;  // (around the end: the fourth pair's upper weight)
+    const uint32_t there = right < 0 ? w << -right : (right == 0 ? w : __builtin_amdgcn_alignbit(w, w, right));
+    b[i] = (there & M::kMask) | base;
   }
   return b;
 }
@@ -432,7 +435,7 @@ head_tile_kernel(const HeadParams p) {
   constexpr int kUnits = WK * P * MT * 256;  // of x per step
   constexpr int kCopies = (kUnits + kLanes - 1) / kLanes, kPlaces = kCopies * kLanes;  // of them per lane; with those too many
   constexpr int kSums = WK * MT * GPC * 4;   // quadruples of row sums per step
-  static_assert(kPlaces < 2 * kUnits && kUnits % 64 == 0 && kSums <= kLanes, "");
+  static_assert(NT * WV <= kTilePadding && kPlaces < 2 * kUnits && kUnits % 64 == 0 && kSums <= kLanes, "");
   constexpr int kOut = WK * WV * 16 * NT * 16;  // floats of 16 rows of the result, per wave
   constexpr int kBytes = 2 * kPlaces * 16 > kOut * 4 ? 2 * kPlaces * 16 : kOut * 4;
   __shared__ __attribute__((aligned(16))) char lds[kBytes];
@@ -454,19 +457,22 @@ head_tile_kernel(const HeadParams p) {
   f32x4 sums_raw;
   RawScales<GPC, ST> s_raw[NT], z_raw[NT];
   // Unit u of a step: chunk u / (256 P MT) of it, 16-row tile u / (256 P) % MT (of those that do not exist the last one).
-  // Everything but the lane's offset is the same in every lane of a wave.
-  const int work_chunks = padded_chunks(p.chunks);
+  // All addresses are a lane's offset from one that is the same in every lane and only moves on from step to step.
+  const uint32_t work_chunks = static_cast<uint32_t>(padded_chunks(p.chunks));
+  uint32_t x_at[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    const int place = i * kLanes + wave * 64, u = kPlaces == kUnits || place < kUnits ? place : place - kUnits;  // (those too many: the first again)
+    const uint32_t tile = static_cast<uint32_t>(min(row_block * MT + u / (256 * P) % MT, row_tiles - 1));
+    x_at[i] = ((tile * work_chunks + u / (256 * P * MT)) * (256 * P) + u % (256 * P) + lane) * 16;
+  }
   const int sum_u = min(tid, kSums - 1);
   const uint32_t sum_at = (static_cast<uint32_t>(min(row_block * MT + sum_u / (GPC * 4) % MT, row_tiles - 1) * work_chunks +
                                                  sum_u / (GPC * 4 * MT)) * (GPC * 4) + sum_u % (GPC * 4)) * 16;
   auto load_step_x = [&](int step) {
+    const char* from = reinterpret_cast<const char*>(p.units) + static_cast<int64_t>(step) * (WK * 256 * P * 16);
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const int place = i * kLanes + wave * 64, u = kPlaces == kUnits || place < kUnits ? place : place - kUnits;  // (those too many: the first again)
-      const int tile = min(row_block * MT + u / (256 * P) % MT, row_tiles - 1);
-      const int64_t unit = (static_cast<int64_t>(tile) * work_chunks + step * WK + u / (256 * P * MT)) * (256 * P) + u % (256 * P);
-      x_raw[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p.units) + unit * 16 + static_cast<uint32_t>(lane * 16));
-    }
+    for (int i = 0; i < kCopies; ++i) x_raw[i] = *reinterpret_cast<const u32x4*>(from + x_at[i]);
     sums_raw = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(p.sums) + static_cast<int64_t>(step) * (WK * GPC * 64) + sum_at);
   };
   auto store_step_x = [&](int buffer) {
@@ -474,21 +480,21 @@ head_tile_kernel(const HeadParams p) {
     for (int i = 0; i < kCopies; ++i) units[buffer * kPlaces + i * kLanes + tid] = x_raw[i];
     sums_lds[buffer][sum_u] = sums_raw;
   };
-  // (all of these offsets but the lane's are the same in every lane)
+  // Tiles behind a chunk's last one are those of the next chunk, or padding; they are not stored.
+  const int64_t chunk_bytes = static_cast<int64_t>(p.tiles) * 1024;
+  constexpr int kScaleTile = kTileRows * GPC * ElemSize<ST>::value;  // bytes of a tile's scales
+  const char* w_from = reinterpret_cast<const char*>(p.blocks) + min(wk, p.chunks - 1) * chunk_bytes + static_cast<int64_t>(tile0) * 1024;
+  const uint32_t w_at = lane * 16, s_at = n * (GPC * ElemSize<ST>::value);
   auto load_step_w = [&](int step) {
     const int chunk = min(step * WK + wk, p.chunks - 1);  // (behind the last one: the last one again)
-    const int64_t block0 = static_cast<int64_t>(chunk) * p.tiles;
-    const int64_t scale0 = GPC > 1 ? block0 : static_cast<int64_t>(chunk_group(p, chunk)) * p.tiles;
+    const int64_t s_from = (static_cast<int64_t>(GPC > 1 ? chunk : chunk_group(p, chunk)) * p.tiles + tile0) * kScaleTile;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const int tile = min(tile0 + i, p.tiles - 1);
-      w_raw[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p.blocks) + (block0 + tile) * 1024 +
-                                                       static_cast<uint32_t>(lane * 16));
-      const int64_t scale_at = (scale0 + tile) * (kTileRows * GPC * ElemSize<ST>::value);
-      s_raw[i] = load_raw_scales<GPC, ST>(static_cast<const char*>(p.scales) + scale_at + static_cast<uint32_t>(n * (GPC * ElemSize<ST>::value)));
-      if (ZEROS)
-        z_raw[i] = load_raw_scales<GPC, ST>(static_cast<const char*>(p.zeros) + scale_at + static_cast<uint32_t>(n * (GPC * ElemSize<ST>::value)));
+      w_raw[i] = *reinterpret_cast<const u32x4*>(w_from + w_at + i * 1024);
+      s_raw[i] = load_raw_scales<GPC, ST>(static_cast<const char*>(p.scales) + s_from + s_at + i * kScaleTile);
+      if (ZEROS) z_raw[i] = load_raw_scales<GPC, ST>(static_cast<const char*>(p.zeros) + s_from + s_at + i * kScaleTile);
     }
+    w_from += (step + 1) * WK + wk < p.chunks ? WK * chunk_bytes : 0;
   };
 
   const uint32_t unpack_base = base_in_register<XT>();
