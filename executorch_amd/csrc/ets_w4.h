@@ -519,7 +519,7 @@ head_tile_kernel(const HeadParams p) {
       float sc[NT], zero[NT];
       // 16 rows after the other (a stage each, for every group): operands are read from LDS kReads products ahead, and
       // while a stage is multiplied the sums of the last one are scaled.
-      constexpr int kStages = GPC * MT, kReads = 2;
+      constexpr int kStages = GPC * MT, kReads = ZEROS && GPC == 1 && MT == 4 && NT == 4 ? 1 : 2;  // (registers)
       u32x4 x[kReads + 1][P];
       constexpr int kBases = (kSteps - 1 + kReads) / kSteps + 1;  // (stages whose operands are being read or multiplied)
       f32x4 acc[2][NT], base[kBases];
