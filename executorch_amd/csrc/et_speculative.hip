@@ -52,7 +52,8 @@ hipError_t launch_verify(ets::VerifyParams p, int num_cus, hipStream_t stream) {
     hipLaunchKernelGGL((ets::verify_greedy_kernel<DT>), dim3(p.sequences), dim3(64 * ets::kDecideWaves), 0, stream, p);
     return hipGetLastError();
   }
-  // With up to two workgroups per CU in verify_rest the decision costs less inside it than a launch would.
+  // With up to two workgroups per CU in verify_rest the decision costs less inside it than a launch would (128256 bf16:
+  // 4 x 4 14.9 us inside, 15.5 with a launch; 16 x 12 40 and 36, 64 x 4 59 and 48).
   const int64_t chunks = static_cast<int64_t>(p.sequences) * p.chunks;
   if (chunks > 2 * num_cus) {
     hipLaunchKernelGGL((ets::verify_decide_kernel<DT>), dim3(p.sequences), dim3(64 * ets::kDecideWaves), 0, stream, p);

@@ -223,7 +223,8 @@ __device__ __forceinline__ double block_sum_f64(double v, double* red) {
 // ---- statistics of every chunk ------------------------------------------------------------------
 // A wave takes one chunk after the other, `stride` of them apart; a chunk is read once, into registers, its
 // maximum found and then its sum, while the next chunk is on its way.  Waves need nothing from each
-// other, so there are no barriers.
+// other, so there are no barriers.  Bound by memory: 64 x 4 at 128256 bf16, 148 MB, in 32 us, 4.6 TB/s (4.9 is what a
+// large copy reaches, 5.95 a kernel that only reads).
 struct ChunkCursor {  // (the same in every lane)
   int b, j, chunk;    // sequence, row of the sequence, chunk of the row
   bool there;         // within the batch
@@ -576,6 +577,9 @@ verify_greedy_kernel(const VerifyParams p) {
 // (rho - rho') B, but for entries whose sign changes between rho and rho'.  Those are among the entries summed up
 // in `edge`, and each is off by at most |rho - rho'| b; verify_finish takes the masses anew with rho' where that
 // could matter (two models that are all but equal).
+//
+// Bound by 64-bit arithmetic, some 25 instructions for each of a row pair's exponentials: 64 pairs of 128256 in 18 us,
+// of which the rows, 33 MB that the statistics have just read, would take 6.
 template <int DT, bool DECIDED>
 __global__ void __launch_bounds__(kVerifyBlock)
 verify_rest_kernel(const VerifyParams p) {
@@ -637,6 +641,8 @@ verify_rest_kernel(const VerifyParams p) {
 }
 
 // ---- the draw -----------------------------------------------------------------------------------
+// A chain of dependent reads and sums, 4 to 6 us whatever the sizes: the masses, the chunk, its 2048 entries.  With 8
+// or 16 waves and fewer entries a lane it was no faster.
 template <int DT>
 __global__ void __launch_bounds__(kVerifyBlock)
 verify_finish_kernel(const VerifyParams p) {

@@ -14,7 +14,8 @@
 // B of the t-th 16x16x32 product), the column 8 q + 2 i + h at bits 16 h + 4 i + 3, around the end of the dword: with
 // bf16 two of its weights are then in place without a shift.  A wave reads a block with one 16-byte load per lane.  The blocks of one chunk of columns are next to each other: workgroups that walk
 // along the columns side by side then read one contiguous stretch of memory at a time, where blocks in row order
-// (32 KiB apart at 4096 columns) would have all of them at the same memory channels (64 rows: 134 us).
+// (32 KiB apart at 4096 columns) would have all of them at the same memory channels (an earlier kernel, 64 rows at
+// 128256 x 4096: 134 us in row order, 112 in this one).
 #pragma once
 
 #include "ets_device.h"
@@ -366,12 +367,20 @@ head_stream_kernel(const HeadParams p) {
 // workgroup makes (16 MT) rows x (16 NT WV) vocabulary entries, WV waves next to each other along the
 // vocabulary, WK behind each other along the columns (each takes every WK-th chunk; their sums are added
 // up in the end).  x goes through LDS, where all waves read it; a wave's weights go from memory to its
-// registers, unpacked there once for all of its rows.
+// registers, unpacked there once for all of its rows.  Weights, x and scales of a step are loaded while the step
+// before is multiplied; one barrier a step.
+//
+// 64 rows at 128256 x 4096: 74 us of head_tile, 0.91 PFLOP/s; 320 rows: 322 us with head_rows, 1.04 PFLOP/s, where a
+// large matrix product of the library reaches 1.38 (and 413 us for these 320 rows with weights of 16 bits).  Bound by
+// the matrix cores with vector instructions beside them (three a product, of unpacking and scaling: two waves of a
+// SIMD then need 1.6 us for 64 x 64 x 128 of each, 1.34 without), and by the reads of x from LDS (10 us of the 74);
+// leaving out the scaling, the unpacking or the reads of weights from memory changes nothing.
 //
 // Work buffer: per 16 rows and chunk of columns, and part of x, 256 units of 16 bytes: row m, columns
 // 32 t + 8 q + 0..7 at unit 16 (4 t + q) + m, so that a wave reads an operand as one contiguous KiB; rows and
 // columns that do not exist are 0.  Behind all of these, per 16 rows and chunk, -24 times the rows' sums of x
 // over each group of the chunk: what the accumulators start from.
+
 // -24 times the sum of the eight columns.
 template <int XT>
 __device__ __forceinline__ float minus24_sum(const RawX<XT>& x) {
@@ -399,7 +408,6 @@ template <int CTRL>
 __device__ __forceinline__ float dpp_add(float v) {
   return v + __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), CTRL, 0xf, 0xf, false));
 }
-
 
 // Chunks of the work buffer: whole rounds of head_tile, whatever its WK; those too many are 0 as well.
 constexpr int kChunkRound = 8;
@@ -519,7 +527,7 @@ head_tile_kernel(const HeadParams p) {
       float sc[NT], zero[NT];
       // 16 rows after the other (a stage each, for every group): operands are read from LDS kReads products ahead, and
       // while a stage is multiplied the sums of the last one are scaled.
-      constexpr int kStages = GPC * MT, kReads = ZEROS && GPC == 1 && MT == 4 && NT == 4 ? 1 : 2;  // (registers)
+      constexpr int kStages = GPC * MT, kReads = ZEROS && GPC == 1 && MT >= 3 && NT == 4 ? 1 : 2;  // (registers)
       u32x4 x[kReads + 1][P];
       constexpr int kBases = (kSteps - 1 + kReads) / kSteps + 1;  // (stages whose operands are being read or multiplied)
       f32x4 acc[2][NT], base[kBases];

@@ -65,7 +65,7 @@ typedef struct ets_verify_batch {
 } ets_verify_batch;
 
 /* Work buffers for calls of at most max_sequences x max_drafts on the current HIP device (about
- * 16 x max_sequences x (2 max_drafts + 2) x vocab / 2048 bytes), allocated here: calls allocate
+ * 16 x max_sequences x (2 max_drafts + 4) x vocab / 2048 bytes), allocated here: calls allocate
  * nothing and may be captured into a graph.  vocab_size is below 16777216. */
 ETS_API ets_status ets_verifier_create(int32_t vocab_size, int32_t max_sequences, int32_t max_drafts, ets_verifier** out);
 ETS_API ets_status ets_verifier_destroy(ets_verifier* v);

@@ -120,6 +120,18 @@ def test_long_vocabularies(dev, dtype, rows, group, zeros):
     check(head.logits(x, dtype=torch.float32), x, w, group, "f32", (dtype, rows, group))
 
 
+@pytest.mark.parametrize("dtype,zeros,group", [("bf16", False, 128), ("f16", True, 64), ("f32", True, 32), ("bf16", True, 128), ("f16", False, 32)])
+@pytest.mark.parametrize("vocab", [20011, 37003, 70001])
+@pytest.mark.parametrize("rows", [20, 40, 64])
+def test_every_size_of_workgroup(dev, dtype, zeros, group, vocab, rows):
+    """Vocabularies that take workgroups of 128, 256 and 512 entries."""
+    hidden = 600
+    w = weights(13, vocab, hidden, group, dtype, zeros, dev)
+    x = states(5, rows, hidden, dtype, dev)
+    head = ea.LogitHead(w[0], w[1], group, zeros=w[2])
+    check(head.logits(x, dtype=torch.float32), x, w, group, "f32", (dtype, rows, vocab))
+
+
 @pytest.mark.parametrize("rows", [1, 20, 100])
 def test_strides_gaps_and_what_lies_beside(dev, rows):
     vocab, hidden, group = 203, 301, 64
