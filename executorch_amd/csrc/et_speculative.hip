@@ -78,7 +78,9 @@ ets_status ets_verifier_create(int32_t vocab_size, int32_t max_sequences, int32_
   if (max_drafts < 0) return verifier_fail(nullptr, ETS_INVALID_ARGUMENT, "ets_verifier_create: max_drafts must be >= 0");
   if (max_drafts > ets::kMaxDrafts) return verifier_fail(nullptr, ETS_NOT_SUPPORTED, "ets_verifier_create: max_drafts must be at most 64");
   const int64_t chunks = chunks_of(vocab_size);
-  if (max_sequences > 65535 || static_cast<int64_t>(max_sequences) * (2 * max_drafts + 1) * chunks > INT32_MAX)
+  // (items and rows are counted in 32 bits; a launch has fewer than 2^32 lanes, of which a sequence's chunk takes 256)
+  if (max_sequences > 65535 || static_cast<int64_t>(max_sequences) * (2 * max_drafts + 1) * chunks > INT32_MAX ||
+      max_sequences * chunks >= (1 << 24))
     return verifier_fail(nullptr, ETS_NOT_SUPPORTED, "ets_verifier_create: max_sequences x max_drafts x vocab_size is too large for one launch");
   ets_verifier* v = new (std::nothrow) ets_verifier();
   if (!v) return verifier_fail(nullptr, ETS_MEMORY_ALLOCATION_FAILED, "ets_verifier_create: out of host memory");

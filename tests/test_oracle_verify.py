@@ -30,7 +30,8 @@ def test_create_refusals_need_no_device():
     for args, code, word in (((0, 1, 1), _capi.INVALID_ARGUMENT, b"vocab_size"), ((10, 0, 1), _capi.INVALID_ARGUMENT, b"max_sequences"),
                              ((10, 1, -1), _capi.INVALID_ARGUMENT, b"max_drafts"), ((10, 1, 65), _capi.NOT_SUPPORTED, b"max_drafts"),
                              ((1 << 24, 1, 1), _capi.NOT_SUPPORTED, b"vocab_size"),
-                             ((1 << 23, 65535, 64), _capi.NOT_SUPPORTED, b"too large")):
+                             ((1 << 23, 65535, 64), _capi.NOT_SUPPORTED, b"too large"),
+                             ((2048 * 257, 65535, 0), _capi.NOT_SUPPORTED, b"too large")):
         assert L.ets_verifier_create(*args, ctypes.byref(h)) == code, args
         assert word in L.ets_verifier_last_error(None), args
     assert L.ets_verifier_create(10, 1, 1, None) == _capi.INVALID_ARGUMENT
