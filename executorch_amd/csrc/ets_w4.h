@@ -368,13 +368,13 @@ head_stream_kernel(const HeadParams p) {
 // vocabulary, WK behind each other along the columns (each takes every WK-th chunk; their sums are added
 // up in the end).  x goes through LDS, where all waves read it; a wave's weights go from memory to its
 // registers, unpacked there once for all of its rows.  Weights, x and scales of a step are loaded while the step
-// before is multiplied; one barrier a step.
+// before is multiplied, and x is stored to LDS beside its last products (behind them: 2 % slower); one barrier a step.
 //
-// 64 rows at 128256 x 4096: 74 us of head_tile, 0.91 PFLOP/s; 320 rows: 322 us with head_rows, 1.04 PFLOP/s, where a
-// large matrix product of the library reaches 1.38 (and 413 us for these 320 rows with weights of 16 bits).  Bound by
-// the matrix cores with vector instructions beside them (three a product, of unpacking and scaling: two waves of a
-// SIMD then need 1.6 us for 64 x 64 x 128 of each, 1.34 without), and by the reads of x from LDS (10 us of the 74);
-// leaving out the scaling, the unpacking or the reads of weights from memory changes nothing.
+// 64 rows at 128256 x 4096: 75 us with head_rows, 0.90 PFLOP/s; 320 rows: 316 us, 1.07 PFLOP/s, where a large matrix
+// product of the library reaches 1.38 (and 413 us for these 320 rows with weights of 16 bits).  Bound by the matrix
+// cores with vector instructions beside them (three a product, of unpacking and scaling: two waves of a SIMD then
+// need 1.6 us for 64 x 64 x 128 of each, 1.34 without), and by the reads of x from LDS (10 us of the 75); leaving out
+// the scaling, the unpacking or the reads of weights from memory changes nothing.
 //
 // Work buffer: per 16 rows and chunk of columns, and part of x, 256 units of 16 bytes: row m, columns
 // 32 t + 8 q + 0..7 at unit 16 (4 t + q) + m, so that a wave reads an operand as one contiguous KiB; rows and
@@ -553,6 +553,7 @@ head_tile_kernel(const HeadParams p) {
 #pragma unroll
       for (int stage = 0; stage < kStages; ++stage) {
         const int g = stage / MT, a = stage % MT;
+        if (stage == kStages - 1) store_step_x(buffer ^ 1);  // (beside the last products; nobody reads that buffer in this step)
         if (a == 0 && g > 0) scale_rows(stage - 1);  // (before the group's scales are replaced)
         if (a == 0) {
 #pragma unroll
@@ -584,8 +585,6 @@ head_tile_kernel(const HeadParams p) {
         __builtin_amdgcn_sched_barrier(0);
       }
       scale_rows(kStages - 1);
-      __builtin_amdgcn_sched_barrier(0);
-      store_step_x(buffer ^ 1);
       __syncthreads();
     }
   }
