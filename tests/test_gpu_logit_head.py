@@ -160,6 +160,30 @@ def test_logits_further_than_31_bits_apart(dev):
     check(ea.LogitHead(w[0], w[1], group).logits(x, out=out), x, w, group, "bf16", "far")
 
 
+@pytest.mark.parametrize("rows,far", [(3, (1 << 30) + 77), (17, (1 << 28) + 3)])
+def test_hidden_states_further_than_31_bits_apart(dev, rows, far):
+    vocab, hidden, group = 100, 384, 128
+    w = weights(42, vocab, hidden, group, "bf16", False, dev)
+    x = states(10, rows, hidden, "bf16", dev)
+    spread = torch.empty((rows - 1) * far + hidden, dtype=torch.bfloat16, device=dev).as_strided((rows, hidden), (far, 1))
+    spread.copy_(x)
+    check(ea.LogitHead(w[0], w[1], group).logits(spread, dtype=torch.float32), x, w, group, "f32", rows)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [2, 4, 5, 6, 16, 17, 33])
+def test_a_last_row_that_is_not_finite(dev, dtype, rows):
+    """The places of rows that do not exist hold copies of the last one."""
+    vocab, hidden, group = 70, 300, 64
+    w = weights(52, vocab, hidden, group, "f32", True, dev)
+    head = ea.LogitHead(w[0], w[1], group, zeros=w[2])
+    x = states(2, rows, hidden, dtype, dev)
+    good = head.logits(x, dtype=torch.float32)
+    x[-1, hidden - 1] = float("nan")
+    bad = head.logits(x, dtype=torch.float32)
+    assert torch.equal(good[:-1], bad[:-1]) and not bad[-1].isfinite().any()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_rows_that_are_not_finite_stay_to_themselves(dev, dtype):
     vocab, hidden, group = 70, 256, 32
@@ -228,6 +252,10 @@ def test_hidden_states_to_tokens(dev):
     assert one.sample_hidden(x[:0], head).shape == (0,)
     before = one.get_rng_states()
     other = ea.Sampler(vocab + 1, 0.7, 0.9, 4, max_batch=rows)
+    for out in (torch.empty(len(x) + 1, dtype=torch.int32, device=dev), torch.empty(len(x), dtype=torch.int64, device=dev),
+                torch.empty(len(x), dtype=torch.int32), torch.empty(2 * len(x), dtype=torch.int32, device=dev)[::2]):
+        with pytest.raises(ea.SamplerError):
+            one.sample_hidden(x, head, out=out)
     for bad in (lambda: other.sample_hidden(x, head), lambda: ea.Sampler(vocab, 0.7, 0.9, 4, max_batch=2).sample_hidden(x, head),
                 lambda: one.sample_hidden(x[:, :-1], head), lambda: one.sample_hidden(x, head, logits=logits[:, :-1])):
         with pytest.raises(ea.SamplerError):
