@@ -58,7 +58,7 @@ hipError_t launch_tiles(const ets::HeadParams& p, hipStream_t stream) {
   // and end; a step of the smallest, half as many products with as many reads of x, takes three quarters of the others'.
   // 64 rows x 4096 columns, us for 512 / 256 / 128 entries: 59 / 37 / 28 at 32000, 61 / 41 / 50 at 64000, 62 / 72 / 94 at
   // 100000, 73 / 82 / 102 at 128256, 126 / 118 / 128 at 151936.
-  constexpr bool kFits = !(ZEROS && GPC == 1 && MT == 4);  // (in the registers, with the copies of two chunks of x)
+  constexpr bool kFits = XT != ets::kDtypeFloat && !(ZEROS && GPC == 1 && MT == 4);  // (in the registers, with two chunks of x)
   constexpr int kCus = 256;
   const int64_t row_blocks = (p.rows + 16 * MT - 1) / (16 * MT);
   auto rounds = [&](int tiles) { return ((p.tiles + tiles - 1) / tiles * row_blocks + kCus - 1) / kCus; };

@@ -93,9 +93,12 @@ __device__ __forceinline__ u32x4 unpack(uint32_t w, uint32_t base) {
   return b;
 }
 
+// Sums are held apart in two: of the highest parts, whose products' few bits add up without a loss as a rule, and of the
+// lower ones, which are 2^-8 of these.  (All in one, the lower parts' last bits are cut off at the ulp of -24 sum x:
+// 6e-7 instead of 1e-7 of a logit.)
 template <int XT>
 struct Parts {
-  static constexpr int value = XT == kDtypeFloat ? 3 : 1;
+  static constexpr int value = XT == kDtypeFloat ? 3 : 1, sums = XT == kDtypeFloat ? 2 : 1;
 };
 
 struct __attribute__((packed, aligned(2))) LooseHalves {
@@ -268,7 +271,9 @@ template <int XT, int GPC, int ST, bool ZEROS, int NT, bool BESIDE>
 __global__ void __launch_bounds__(kHeadBlock)
 head_stream_kernel(const HeadParams p) {
   using M = Matrix<XT>;
-  constexpr int P = BESIDE ? 1 : Parts<XT>::value, kWavesHere = kHeadBlock / 64, kSteps = 4 / GPC;  // products per group of a chunk
+  constexpr int P = BESIDE ? 1 : Parts<XT>::value, S = BESIDE ? 1 : Parts<XT>::sums;
+  constexpr int kWavesHere = kHeadBlock / 64, kSteps = 4 / GPC;  // products per group of a chunk
+  constexpr auto sum_of = [](int part) { return part == 0 ? 0 : S - 1; };
   __shared__ float red[kWavesHere][NT][64 * 4];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, q = lane >> 4;
   const int tile0 = blockIdx.x * NT, m0 = blockIdx.y * 16;
@@ -313,28 +318,30 @@ head_stream_kernel(const HeadParams p) {
     }
 #pragma unroll
     for (int g = 0; g < GPC; ++g) {
-      f32x4 base = {0.0f, 0.0f, 0.0f, 0.0f};
+      f32x4 base[S] = {};
 #pragma unroll
       for (int t = g * kSteps; t < (g + 1) * kSteps; ++t) {
 #pragma unroll
-        for (int k = 0; k < P; ++k) base = M::product(x[t][k], minus24, base);
+        for (int k = 0; k < P; ++k) base[sum_of(k)] = M::product(x[t][k], minus24, base[sum_of(k)]);
       }
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        f32x4 acc = base;
+        f32x4 acc[S];
+#pragma unroll
+        for (int c = 0; c < S; ++c) acc[c] = base[c];
 #pragma unroll
         for (int t = g * kSteps; t < (g + 1) * kSteps; ++t) {
           const u32x4 b = unpack<XT>(w[i][t], unpack_base);
 #pragma unroll
-          for (int k = 0; k < P; ++k) acc = M::product(x[t][k], b, acc);
+          for (int k = 0; k < P; ++k) acc[sum_of(k)] = M::product(x[t][k], b, acc[sum_of(k)]);
         }
         const float scale = scale_of<GPC, ST>(s[i], g, ~0u);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) total[i][r] = fmaf(scale, acc[r], total[i][r]);
+        for (int r = 0; r < 4; ++r) total[i][r] = fmaf(scale, S == 1 ? acc[0][r] : acc[0][r] + acc[S - 1][r], total[i][r]);
         if (ZEROS) {
           const float zero = scale_of<GPC, ST>(z[i], g, ~0u) * (-1.0f / 24.0f);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) total[i][r] = fmaf(zero, base[r], total[i][r]);
+          for (int r = 0; r < 4; ++r) total[i][r] = fmaf(zero, S == 1 ? base[0][r] : base[0][r] + base[S - 1][r], total[i][r]);
         }
       }
     }
@@ -379,17 +386,25 @@ head_stream_kernel(const HeadParams p) {
 // Work buffer: per 16 rows and chunk of columns, and part of x, 256 units of 16 bytes: row m, columns
 // 32 t + 8 q + 0..7 at unit 16 (4 t + q) + m, so that a wave reads an operand as one contiguous KiB; rows and
 // columns that do not exist are 0.  Behind all of these, per 16 rows and chunk, -24 times the rows' sums of x
-// over each group of the chunk: what the accumulators start from.
+// over each group of the chunk (of fp32 the highest parts' sums, then the others'): what the accumulators start from.
 
-// -24 times the sum of the eight columns.
+// -24 times the sums of the eight columns (of fp32: of their highest parts, and of what is left of them).
 template <int XT>
-__device__ __forceinline__ float minus24_sum(const RawX<XT>& x) {
-  float s = 0.0f;
+__device__ __forceinline__ void minus24_sums(const RawX<XT>& x, float* sums) {
   if (XT == kDtypeFloat) {
+    float high = 0.0f, rest = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s += __uint_as_float(x.v[j >> 2][j & 3]);
-    return -24.0f * s;
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t bits = x.v[(j >> 2) * (XT == kDtypeFloat)][j & 3];
+      const float h = __uint_as_float(bits & 0xffff0000u);
+      high += h;
+      rest += __uint_as_float(bits) - h;
+    }
+    sums[0] = -24.0f * high;
+    sums[Parts<XT>::sums - 1] = -24.0f * rest;
+    return;
   }
+  float s = 0.0f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t pair = x.v[0][i];  // (a bit cast of the vector's element itself takes its first element)
@@ -401,7 +416,7 @@ __device__ __forceinline__ float minus24_sum(const RawX<XT>& x) {
       s = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), f16x2{static_cast<_Float16>(-24.0f), static_cast<_Float16>(-24.0f)}, s, false);
     }
   }
-  return s;
+  sums[0] = s;
 }
 
 template <int CTRL>
@@ -416,7 +431,7 @@ __host__ __device__ __forceinline__ int padded_chunks(int chunks) { return (chun
 template <int XT, int GPC>
 __global__ void __launch_bounds__(kHeadBlock)
 head_rows_kernel(const void* x, int64_t x_stride, int32_t rows, int32_t hidden, u32x4* units, float* sums) {
-  constexpr int P = Parts<XT>::value;
+  constexpr int P = Parts<XT>::value, S = Parts<XT>::sums;
   const int slot = threadIdx.x & 15, in_tile = threadIdx.x >> 4, chunk = blockIdx.x, m = blockIdx.y * 16 + in_tile;
   const bool exists = m < rows;
   const char* row = static_cast<const char*>(x) + (exists ? m : 0) * x_stride * ElemSize<XT>::value;
@@ -427,22 +442,28 @@ head_rows_kernel(const void* x, int64_t x_stride, int32_t rows, int32_t hidden, 
   const int64_t block = static_cast<int64_t>(blockIdx.y) * gridDim.x + chunk;
 #pragma unroll
   for (int c = 0; c < P; ++c) units[(block * P + c) * 256 + slot * 16 + in_tile] = part[c];
-  float s = minus24_sum<XT>(raw);  // the 16 lanes of a row hold its chunk
-  s = dpp_add<0xb1>(s);
-  s = dpp_add<0x4e>(s);
-  if (GPC <= 2) s = dpp_add<0x141>(s);
-  if (GPC == 1) s = dpp_add<0x140>(s);
-  if (slot % (16 / GPC) == 0) sums[(block * GPC + slot / (16 / GPC)) * 16 + in_tile] = s;
+  float s[S];
+  minus24_sums<XT>(raw, s);  // the 16 lanes of a row hold its chunk
+#pragma unroll
+  for (int c = 0; c < S; ++c) {
+    s[c] = dpp_add<0xb1>(s[c]);
+    s[c] = dpp_add<0x4e>(s[c]);
+    if (GPC <= 2) s[c] = dpp_add<0x141>(s[c]);
+    if (GPC == 1) s[c] = dpp_add<0x140>(s[c]);
+    if (slot % (16 / GPC) == 0) sums[((block * S + c) * GPC + slot / (16 / GPC)) * 16 + in_tile] = s[c];
+  }
 }
 
 template <int XT, int GPC, int ST, bool ZEROS, int MT, int NT, int WV, int WK>
 __global__ void __launch_bounds__(64 * WV * WK, 2)
 head_tile_kernel(const HeadParams p) {
   using M = Matrix<XT>;
-  constexpr int P = Parts<XT>::value, kSteps = 4 / GPC, kLanes = 64 * WV * WK, kRows = 16 * MT;
+  constexpr int P = Parts<XT>::value, S = Parts<XT>::sums, kSteps = 4 / GPC, kLanes = 64 * WV * WK, kRows = 16 * MT;
+  constexpr auto sum_of = [](int part) { return part == 0 ? 0 : S - 1; };
+  constexpr int kSumUnits = S * GPC * 4;     // quadruples of row sums of 16 rows and a chunk
   constexpr int kUnits = WK * P * MT * 256;  // of x per step
   constexpr int kCopies = (kUnits + kLanes - 1) / kLanes, kPlaces = kCopies * kLanes;  // of them per lane; with those too many
-  constexpr int kSums = WK * MT * GPC * 4;   // quadruples of row sums per step
+  constexpr int kSums = WK * MT * kSumUnits; // of them per step
   static_assert(NT * WV <= kTilePadding && kPlaces < 2 * kUnits && kUnits % 64 == 0 && kSums <= kLanes, "");
   constexpr int kOut = WK * WV * 16 * NT * 16;  // floats of 16 rows of the result, per wave
   constexpr int kBytes = 2 * kPlaces * 16 > kOut * 4 ? 2 * kPlaces * 16 : kOut * 4;
@@ -475,13 +496,13 @@ head_tile_kernel(const HeadParams p) {
     x_at[i] = ((tile * work_chunks + u / (256 * P * MT)) * (256 * P) + u % (256 * P) + lane) * 16;
   }
   const int sum_u = min(tid, kSums - 1);
-  const uint32_t sum_at = (static_cast<uint32_t>(min(row_block * MT + sum_u / (GPC * 4) % MT, row_tiles - 1) * work_chunks +
-                                                 sum_u / (GPC * 4 * MT)) * (GPC * 4) + sum_u % (GPC * 4)) * 16;
+  const uint32_t sum_at = (static_cast<uint32_t>(min(row_block * MT + sum_u / kSumUnits % MT, row_tiles - 1) * work_chunks +
+                                                 sum_u / (kSumUnits * MT)) * kSumUnits + sum_u % kSumUnits) * 16;
   auto load_step_x = [&](int step) {
     const char* from = reinterpret_cast<const char*>(p.units) + static_cast<int64_t>(step) * (WK * 256 * P * 16);
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) x_raw[i] = *reinterpret_cast<const u32x4*>(from + x_at[i]);
-    sums_raw = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(p.sums) + static_cast<int64_t>(step) * (WK * GPC * 64) + sum_at);
+    sums_raw = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(p.sums) + static_cast<int64_t>(step) * (WK * kSumUnits * 16) + sum_at);
   };
   auto store_step_x = [&](int buffer) {
 #pragma unroll
@@ -530,10 +551,13 @@ head_tile_kernel(const HeadParams p) {
       constexpr int kStages = GPC * MT, kReads = ZEROS && GPC == 1 && MT >= 3 && NT == 4 ? 1 : 2;  // (registers)
       u32x4 x[kReads + 1][P];
       constexpr int kBases = (kSteps - 1 + kReads) / kSteps + 1;  // (stages whose operands are being read or multiplied)
-      f32x4 acc[2][NT], base[kBases];
+      f32x4 acc[2][S][NT], base[kBases][S];
       auto read_x = [&](int at) {  // operand t of a stage: at = stage * kSteps + t
         const int stage = at / kSteps, g = stage / MT, a = stage % MT, t = at % kSteps;
-        if (t == 0) base[stage % kBases] = sums_lds[buffer][((wk * MT + a) * GPC + g) * 4 + q];
+        if (t == 0) {
+#pragma unroll
+          for (int c = 0; c < S; ++c) base[stage % kBases][c] = sums_lds[buffer][((wk * MT + a) * S + c) * (GPC * 4) + g * 4 + q];
+        }
 #pragma unroll
         for (int c = 0; c < P; ++c)
           x[at % (kReads + 1)][c] = units[buffer * kPlaces + ((wk * MT + a) * P + c) * 256 + (g * kSteps + t) * 64 + lane];
@@ -543,7 +567,10 @@ head_tile_kernel(const HeadParams p) {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) total[a][i][r] = fmaf(sc[i], acc[stage & 1][i][r], total[a][i][r]);
+          for (int r = 0; r < 4; ++r) {
+            const float sum = S == 1 ? acc[stage & 1][0][i][r] : acc[stage & 1][0][i][r] + acc[stage & 1][S - 1][i][r];
+            total[a][i][r] = fmaf(sc[i], sum, total[a][i][r]);
+          }
         // (pinned here: left alone, the compiler gathers all of a chunk's scaling behind all of its products, and spills)
 #pragma unroll
         for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(total[a][i]));
@@ -570,15 +597,20 @@ head_tile_kernel(const HeadParams p) {
           for (int i = 0; i < NT; ++i) {
             if (a == 0) b[i][t] = unpack<XT>(w_raw[i][g * kSteps + t], unpack_base);
 #pragma unroll
-            for (int c = 0; c < P; ++c)
-              acc[stage & 1][i] = M::product(x[at % (kReads + 1)][c], b[i][t], t == 0 && c == 0 ? base[stage % kBases] : acc[stage & 1][i]);
+            for (int c = 0; c < P; ++c) {
+              f32x4& sum = acc[stage & 1][sum_of(c)][i];
+              sum = M::product(x[at % (kReads + 1)][c], b[i][t], t == 0 && c <= 1 ? base[stage % kBases][sum_of(c)] : sum);
+            }
           }
         }
         if (ZEROS) {
 #pragma unroll
           for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) total[a][i][r] = fmaf(zero[i], base[stage % kBases][r], total[a][i][r]);
+            for (int r = 0; r < 4; ++r) {
+              const f32x4* from = base[stage % kBases];
+              total[a][i][r] = fmaf(zero[i], S == 1 ? from[0][r] : from[0][r] + from[S - 1][r], total[a][i][r]);
+            }
         }
         if (a == 0 && g == GPC - 1) load_step_w(step + 1);
         if (a > 0) scale_rows(stage - 1);

@@ -160,6 +160,27 @@ def test_logits_further_than_31_bits_apart(dev):
     check(ea.LogitHead(w[0], w[1], group).logits(x, out=out), x, w, group, "bf16", "far")
 
 
+@pytest.mark.parametrize("group", [32, 128, 1 << 20])
+@pytest.mark.parametrize("rows", [1, 5, 6, 16, 17, 64])
+def test_states_of_32_bits_keep_them(dev, rows, group):
+    """The sums of fp32 states: with scales of 1 a logit is an integer combination of 24-bit numbers.  Held apart, the highest
+    parts add up exactly (8 bits times 5, over 640 columns, within the 24 of a sum, as long as x stays within a few binades)
+    and the lower ones lose at most their own 2^-24 per addition: 2^-8 of what one sum for all would."""
+    vocab, hidden = 80, 640
+    g = np.random.default_rng(rows)
+    packed = torch.from_numpy(g.integers(0, 256, size=(vocab, hidden // 2), dtype=np.uint8)).to(dev)
+    scales = torch.ones((vocab, -(-hidden // group)), device=dev)
+    x = torch.from_numpy((1 + g.random((rows, hidden))).astype(np.float32)).to(dev)
+    y = ea.LogitHead(packed, scales, group).logits(x).double().cpu().numpy()
+    want, _ = HO.logits(host(x), packed.cpu().numpy(), host(scales), None, group, "f32")
+    # lower parts: below 2^-7 each, times at most 31, 1280 products and their start, each sum cut at 2^-23 of the largest
+    # partial sum, 640 x 31 x 2^-7; a group's two sums added, and the groups' sums: 2^-24 of |y| and of the largest group sum
+    # (640 x 8 x 2 at most) each
+    most = 640 * 8 * 2.0
+    bound = (3 * 640 / 8) * 2.0 ** -23 * (640 * 31 * 2.0 ** -7) + 2 * (-(-hidden // group)) * 2.0 ** -24 * most
+    assert np.abs(y - want).max() <= bound
+
+
 @pytest.mark.parametrize("rows,far", [(3, (1 << 30) + 77), (17, (1 << 28) + 3)])
 def test_hidden_states_further_than_31_bits_apart(dev, rows, far):
     vocab, hidden, group = 100, 384, 128
