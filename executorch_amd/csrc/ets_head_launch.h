@@ -53,21 +53,26 @@ hipError_t launch_tiles(const ets::HeadParams& p, hipStream_t stream) {
 
 template <int XT, int GPC, int ST, bool ZEROS, int MT>
 hipError_t launch_tiles(const ets::HeadParams& p, hipStream_t stream) {
-  // Workgroups of 512, 256 or 128 vocabulary entries.  Each of the 256 CUs takes one at a time, so rounds count.  A round
+  // Workgroups of 512, 256, 128 or 64 vocabulary entries.  Each of the 256 CUs takes one at a time, so rounds count.  A round
   // takes as many steps as there are chunks of columns for a wave (WK waves share them), and about three more for its start
-  // and end; a step of the smallest, half as many products with as many reads of x, takes three quarters of the others'.
-  // 64 rows x 4096 columns, us for 512 / 256 / 128 entries: 59 / 37 / 28 at 32000, 61 / 41 / 50 at 64000, 62 / 72 / 94 at
-  // 100000, 73 / 82 / 102 at 128256, 126 / 118 / 128 at 151936.
-  constexpr bool kFits = XT != ets::kDtypeFloat && !(ZEROS && GPC == 1 && MT == 4);  // (in the registers, with two chunks of x)
+  // and end; a step of 128 entries, half as many products with as many reads of x, takes three quarters of the others'.
+  // 64 rows x 4096 columns, us for 512 / 256 / 128 / 64 entries: 59 / 37 / 26 / 20 at 4000, 59 / 37 / 28 / - at 32000,
+  // 61 / 41 / 50 / - at 64000, 62 / 72 / 94 / - at 100000, 73 / 82 / 102 / - at 128256, 126 / 118 / 128 / - at 151936.
+  // Without 256 where two chunks of x do not fit the registers, without 64 where four do not fit LDS (three parts each).
+  constexpr bool kMiddle = XT != ets::kDtypeFloat && !(ZEROS && GPC == 1 && MT == 4), kTiny = XT != ets::kDtypeFloat;
   constexpr int kCus = 256;
   const int64_t row_blocks = (p.rows + 16 * MT - 1) / (16 * MT);
   auto rounds = [&](int tiles) { return ((p.tiles + tiles - 1) / tiles * row_blocks + kCus - 1) / kCus; };
   const int64_t large = rounds(32) * (4 * p.chunks + 12), small = rounds(8) * (3 * ((p.chunks + 1) / 2) + 12);
-  if constexpr (kFits) {
-    const int64_t middle = rounds(16) * (4 * ((p.chunks + 1) / 2) + 12);
-    if (middle < large && middle < small) return launch_tiles<XT, GPC, ST, ZEROS, MT, 4, 4, 2>(p, stream);
+  const int64_t middle = rounds(16) * (4 * ((p.chunks + 1) / 2) + 12), tiny = rounds(4) * (4 * ((p.chunks + 3) / 4) + 12);
+  const int64_t least = small < large ? small : large;
+  if constexpr (kMiddle) {
+    if (middle < least && middle <= tiny) return launch_tiles<XT, GPC, ST, ZEROS, MT, 4, 4, 2>(p, stream);
   }
-  return small < large ? launch_tiles<XT, GPC, ST, ZEROS, MT, 2, 4, 2>(p, stream) : launch_tiles<XT, GPC, ST, ZEROS, MT, 4, 8, 1>(p, stream);
+  if constexpr (kTiny) {
+    if (tiny < least) return launch_tiles<XT, GPC, ST, ZEROS, MT, 2, 2, 4>(p, stream);
+  }
+  return small == least ? launch_tiles<XT, GPC, ST, ZEROS, MT, 2, 4, 2>(p, stream) : launch_tiles<XT, GPC, ST, ZEROS, MT, 4, 8, 1>(p, stream);
 }
 
 template <int XT, int GPC, int ST, bool ZEROS>

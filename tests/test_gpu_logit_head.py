@@ -121,10 +121,10 @@ def test_long_vocabularies(dev, dtype, rows, group, zeros):
 
 
 @pytest.mark.parametrize("dtype,zeros,group", [("bf16", False, 128), ("f16", True, 64), ("f32", True, 32), ("bf16", True, 128), ("f16", False, 32)])
-@pytest.mark.parametrize("vocab", [20011, 37003, 70001])
+@pytest.mark.parametrize("vocab", [9001, 20011, 37003, 70001])
 @pytest.mark.parametrize("rows", [20, 40, 64])
 def test_every_size_of_workgroup(dev, dtype, zeros, group, vocab, rows):
-    """Vocabularies that take workgroups of 128, 256 and 512 entries."""
+    """Vocabularies that take workgroups of 64, 128, 256 and 512 entries."""
     hidden = 600
     w = weights(13, vocab, hidden, group, dtype, zeros, dev)
     x = states(5, rows, hidden, dtype, dev)
